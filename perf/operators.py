@@ -82,8 +82,8 @@ def _side(rng, lo, hi):
 def _draw_one(rng):
     kind = rng.choices(("norm", "train", "store", "layer", "block"), (3, 4, 2, 3, 2))[0]
     dtype = rng.choices(("float32", "bfloat16", "float16", "float64"), (6, 3, 1.5, 1))[0]
-    N, C, H = _log(rng, 1, 32), _log(rng, 4, 512), _side(rng, 1, 512)
-    W = H if rng.random() < 0.4 else _side(rng, max(1, int(H * 0.6)), max(2, int(H * 1.7)))
+    N, C, H = _log(rng, 1, 32), _log(rng, 4, 512), _side(rng, 2, 512)
+    W = H if rng.random() < 0.4 else _side(rng, max(2, int(H * 0.6)), max(3, int(H * 1.7)))
     if kind in ("norm", "train"):
         tokens = rng.random() < 0.3
         if tokens:
@@ -100,7 +100,7 @@ def _draw_one(rng):
 
 
 def draw(rng):
-    """One more case: 1 to 32 images of 4 to 512 channels and sides of 1 to 512, or 1 to 65536 rows of 8 to 8192 channels, every
+    """One more case: 1 to 32 images of 4 to 512 channels and sides of 2 to 512, or 1 to 65536 rows of 8 to 8192 channels, every
     type, with and without residual; layers of 1 to 64 channels and structuring elements of 3 x 3 to 7 x 7. At most 100 M elements a
     tensor (a quarter of that in double), 220 M taps a layer."""
     while True:
