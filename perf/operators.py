@@ -296,12 +296,13 @@ def _morph(x, w, op, merge):
 
 def _morph_backward(x, w, op, merge, gz):
     identity = merge == "identity"
-    place, _ = _positions(*x.shape[2:], w.shape[-1], x.device)
+    place, inside = _positions(*x.shape[2:], w.shape[-1], x.device)
     won = _winners(_tap_values(x, w, op, place, identity), op)
     share = won * _spread(gz, merge, x.shape[1])
     gw = share.sum((0, 4), dtype=torch.float64)
     gw = -gw.flip(2) if op == "erosion" else gw
-    return _scattered(share, place, x, identity), gw.view(w.shape)
+    # A winning tap outside the image, which read the nearest edge pixel, counts for the weight alone.
+    return _scattered(share * inside, place, x, identity), gw.view(w.shape)
 
 
 def _tilde(w, alpha):
@@ -443,20 +444,15 @@ def _unfolded(x, k, replicate):
     return windows.flip(4, 5).permute(0, 1, 4, 5, 2, 3).reshape(N, C, k * k, H, W)
 
 
-def _folded(taps, H, W, k, replicate):
-    """The transpose of _unfolded: [N, C, taps, H, W] back onto [N, C, H, W]."""
+def _folded(taps, H, W, k):
+    """Adds [N, C, taps, H, W] at the pixels of [N, C, H, W] that the taps read; those outside the image are lost."""
     N, C = taps.shape[:2]
-    before, after = k - 1 - k // 2, k // 2
+    before = k - 1 - k // 2
     padded = torch.zeros(N, C, H + k - 1, W + k - 1, dtype=taps.dtype, device=taps.device)
     for tap in range(k * k):
         kh, kw = k - 1 - tap // k, k - 1 - tap % k
         padded[:, :, kh:kh + H, kw:kw + W] += taps[:, :, tap]
-    if not replicate:
-        return padded[:, :, before:before + H, before:before + W]
-    rows = torch.arange(-before, H + after, device=taps.device).clamp(0, H - 1)
-    cols = torch.arange(-before, W + after, device=taps.device).clamp(0, W - 1)
-    out = torch.zeros(N, C, H, W + k - 1, dtype=taps.dtype, device=taps.device).index_add_(2, rows, padded)
-    return torch.zeros(N, C, H, W, dtype=taps.dtype, device=taps.device).index_add_(3, cols, out)
+    return padded[:, :, before:before + H, before:before + W]
 
 
 def _exact_layer(s, x, kept):
@@ -503,7 +499,7 @@ def _exact_layer(s, x, kept):
         share = torch.where(k * k - order == first, gz, 0.0)
         gw = sign * share.sum((0, 4, 5)).view(w.shape)
         more = (torch.flip(gw, (2, 3)) if op == "erosion" else gw,)
-    gx = _folded(share.sum(2) if identity else share.sum(1), H, W, k, op != "smorph")
+    gx = _folded(share.sum(2) if identity else share.sum(1), H, W, k)
     return z, gx, more
 
 
