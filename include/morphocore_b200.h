@@ -51,7 +51,9 @@ enum mc_pad_kind { MC_PAD_FILL = 0, MC_PAD_REPLICATE = 1 };
  * ACCUMULATE: the backward functions add to what gx and gw hold instead of overwriting them (the forward functions ignore it). */
 enum mc_flags { MC_FLAG_FLIPPED_WEIGHT = 1, MC_FLAG_ACCUMULATE = 2 };
 
-enum mc_dtype { MC_F32 = 0, MC_F64 = 1 };
+/* F16 and BF16 exist for mc_encode8, mc_decode8 and mc_rms_norm_* only, which read and write them as they are; the other
+ * functions refuse them. */
+enum mc_dtype { MC_F32 = 0, MC_F64 = 1, MC_F16 = 2, MC_BF16 = 3 };
 
 enum mc_status
 {
@@ -104,7 +106,8 @@ size_t mc_morpho_backward_workspace_bytes(const mc_desc* desc, int have_idx);
 
 /* Backward dilation / erosion. Replaces morpho_backward_cuda<op, T> (CU/morpho_op.cuh:21-24,
  * CU/morpho_op.cu:102-177). gx [B,Ci,H,W] and gw (shape of the shared structuring element) are
- * overwritten (zeroed then accumulated; only accumulated with MC_FLAG_ACCUMULATE). idx is the tensor written by mc_morpho_forward or NULL. */
+ * overwritten (zeroed then accumulated; only accumulated with MC_FLAG_ACCUMULATE). idx is the tensor written by mc_morpho_forward or NULL. x is not
+ * read, and may be NULL, where a MAX / MIN merge is given its idx. */
 int mc_morpho_backward(const mc_desc* desc, const void* x, const void* w, const int32_t* idx, const void* gy, void* gx, void* gw,
                        void* workspace, size_t workspace_bytes, void* stream);
 
@@ -134,7 +137,7 @@ int mc_smorph_forward(const mc_desc* desc, const void* x, const void* w, const v
 size_t mc_smorph_backward_workspace_bytes(const mc_desc* desc);
 
 /* Backward smorph. Replaces smorph_backward_cuda<T> (CU/smorph.cuh:20-25, CU/smorph.cu:63-103).
- * y is the forward output (the merge target of MAX / MIN). gx, gw and galpha_pairs (one value per pair,
+ * y is the forward output: the merge target of MAX / MIN, not read (it may be NULL) for the other merges. gx, gw and galpha_pairs (one value per pair,
  * like alpha_pairs) are overwritten. */
 int mc_smorph_backward(const mc_desc* desc, const void* x, const void* w, const void* alpha_pairs, const void* y, const void* gy, void* gx,
                        void* gw, void* galpha_pairs, void* workspace, size_t workspace_bytes, void* stream);
@@ -165,6 +168,60 @@ size_t mc_smorph_scm_backward_workspace_bytes(const mc_desc* desc);
 int mc_smorph_scm_backward(const mc_desc* desc, const void* x, const void* w, const void* alpha_pairs, const void* beta, const void* y,
                            const void* gy, void* gx, void* gw, void* galpha_pairs, void* gbeta, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* ---- Activations in 8 bits (no counterpart in the reference) --------------------------------------------------------
+ *
+ * A tensor is seen as `rows` rows of `length` consecutive elements (a plane of H x W pixels, or the channels of a token), and
+ * each row as blocks of MC_CODE_BLOCK elements, the last one shorter. A block is stored as one int8 code an element and one
+ * scale: with m the largest finite magnitude of the block,
+ *     scale = m * (1 / 126), code = x * (126 / m) rounded to the nearest whole number (ties to even), value = code * scale,
+ * where 1 / 126 and 126 / m are held in the type of the scales, and the product with x is rounded once. Codes of finite values
+ * are -126 .. 126; -128 stands for NaN, -127 and 127 for the infinities, so that a masked or padded element neither spoils its
+ * block nor comes back as a number. A block whose m lies below 2^-100 (2^-900 in double) is stored as zeros. A finite value comes
+ * back within scale / 2 and a few units in its last place. The scales are float, [rows, ceil(length / MC_CODE_BLOCK)], or
+ * double for MC_F64. Encoding what mc_decode8 gave returns the same values to the last place or two. */
+#define MC_CODE_BLOCK 128
+
+typedef struct mc_rows_desc
+{
+    int64_t rows, length;
+    int32_t dtype;    /* mc_dtype of the tensor */
+    int32_t reserved; /* 0 */
+} mc_rows_desc;
+
+int mc_encode8(const mc_rows_desc* desc, const void* x, int8_t* codes, void* scales, void* stream);
+int mc_decode8(const mc_rows_desc* desc, const int8_t* codes, const void* scales, void* x, void* stream);
+
+/* ---- Root-mean-square norm (no counterpart in the reference) ------------------------------------------------------------
+ *
+ * Tensors are [outer, channels, inner], contiguous: (N, C, H * W) for feature maps, (tokens, C, 1) for rows of channels. With
+ * s = x + residual rounded to the tensors' type (s = x where there is no residual),
+ *     y = s * r * weight[c], r = 1 / sqrt(mean over the channels of s^2 + eps),
+ * the mean and r held in double. y and the 8-bit forms are optional (NULL), at least one output is not. The 8-bit form is that of
+ * mc_encode8 applied to y, or to s, with rows of `inner` elements, or of `channels` where inner is 1: it is what a layer behind
+ * the norm, or the norm itself, may keep for its backward pass instead of the tensor.
+ * `sum` receives s; it is required with a residual and must be NULL without. Buffers that are read may not overlap those
+ * that are written. */
+typedef struct mc_norm_desc
+{
+    int64_t outer, channels, inner;
+    double eps;       /* > 0 */
+    int32_t dtype;    /* mc_dtype of every tensor; r and the sums are wider */
+    int32_t reserved; /* 0 */
+} mc_norm_desc;
+
+int mc_rms_norm_forward(const mc_norm_desc* desc, const void* x, const void* residual, const void* weight, void* sum, void* y, int8_t* y_codes,
+                        void* y_scales, int8_t* sum_codes, void* sum_scales, void* stream);
+
+/* Scratch bytes mc_rms_norm_backward needs: partial sums of the weight's gradient, 0 where gweight is not asked for. */
+size_t mc_rms_norm_backward_workspace_bytes(const mc_norm_desc* desc, int have_gweight);
+
+/* Gradients at s, given as `sum` or (sum NULL) as its 8-bit form: with u = gy * weight[c],
+ *     gx = r * (u - s r^2 mean over the channels of (u s)) + gsum, gweight[c] = sum over all but the channels of gy s r.
+ * gx is the gradient of x and of the residual alike. gsum (nullable) is the gradient of the forward function's `sum`. weight
+ * and gweight are NULL together or not. Results do not depend on the order in which the hardware runs the thread blocks. */
+int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t* sum_codes, const void* sum_scales, const void* weight, const void* gy,
+                         const void* gsum, void* gx, void* gweight, void* workspace, size_t workspace_bytes, void* stream);
 
 const char* mc_status_string(int status);
 const char* mc_last_error(void);

@@ -192,7 +192,9 @@ int mc_morpho_backward(const mc_desc* desc, const void* x, const void* w, const 
         if (cudaMemsetAsync(gw, 0, wn * (desc->dtype == MC_F32 ? 4 : 8), s) != cudaSuccess) { set_last_error("cudaMemsetAsync failed"); return MC_ERR_CUDA; }
         return MC_OK;
     }
-    MC_REQUIRE(x); MC_REQUIRE(w); MC_REQUIRE(gy); MC_REQUIRE(gx);
+    const bool winners_known = idx != nullptr && (desc->merge == MC_MERGE_MAX || desc->merge == MC_MERGE_MIN);
+    if (!winners_known) MC_REQUIRE(x);
+    MC_REQUIRE(w); MC_REQUIRE(gy); MC_REQUIRE(gx);
     const size_t need = mc_morpho_backward_workspace_bytes(desc, idx != nullptr);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     {
@@ -247,7 +249,8 @@ int mc_smorph_backward(const mc_desc* desc, const void* x, const void* w, const 
         }
         return MC_OK;
     }
-    MC_REQUIRE(x); MC_REQUIRE(w); MC_REQUIRE(alpha_pairs); MC_REQUIRE(y); MC_REQUIRE(gy); MC_REQUIRE(gx);
+    MC_REQUIRE(x); MC_REQUIRE(w); MC_REQUIRE(alpha_pairs); MC_REQUIRE(gy); MC_REQUIRE(gx);
+    if (desc->merge == MC_MERGE_MAX || desc->merge == MC_MERGE_MIN) MC_REQUIRE(y);
     const size_t need = mc_smorph_backward_workspace_bytes(desc);
     if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     {

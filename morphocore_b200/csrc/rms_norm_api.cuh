@@ -1,0 +1,30 @@
+// What the entry points of the root-mean-square norm share with its per-type translation units.
+#pragma once
+#include "encode8.cuh"
+
+namespace mc
+{
+
+struct NormArgs;
+struct NormGradArgs;
+
+template <typename T> int rms_norm_forward(const NormArgs& a, cudaStream_t stream);
+template <typename T> int rms_norm_backward(const NormGradArgs& a, cudaStream_t stream);
+
+/// Thread blocks of the backward kernels, each of which leaves one row of partial sums of gweight. They walk over the tiles (or
+/// rows): more of them than are resident would only add rows.
+inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner)
+{
+    constexpr int64_t SMS = 148;
+    if (inner != 1)
+    {
+        const int64_t tiles = outer * code_blocks(inner);
+        return std::min(tiles, SMS * (channels <= 64 ? 3 : 2));
+    }
+    const int64_t blocks = code_blocks(channels);
+    int64_t groups = 8;   // rows that a thread block has at work
+    while (groups > 1 && blocks * groups > 32) groups /= 2;
+    return std::min((outer + groups - 1) / groups, SMS * (blocks > 32 ? 1 : 3));
+}
+
+}  // namespace mc

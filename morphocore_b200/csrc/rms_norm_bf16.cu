@@ -1,0 +1,2 @@
+#define MC_T __nv_bfloat16
+#include "rms_norm_inst.cuh"

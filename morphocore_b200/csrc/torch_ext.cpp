@@ -1,5 +1,5 @@
 // Thin PyTorch extension: registers torch.ops.morphocore.{dilation, erosion, smorph, smorph_scm} with the
-// reference's schemas (morphocore/functional/csrc/cpp/bindings.cpp:130-148) and forwards them, through two
+// reference's schemas (morphocore/functional/csrc/cpp/bindings.cpp:130-148) and forwards them, through their
 // autograd Functions, to the C-ABI of include/morphocore_b200.h. It mirrors the reference wrappers
 // (csrc/cpp/morpho_op_wrap.hxx:25-211, csrc/cpp/smorph.cpp:21-111): 2-D / 3-D inputs and 2-D weights are
 // lifted to 4-D, the same checks raise the same messages, the wrapper owns every allocation and the
@@ -101,6 +101,123 @@ double fill_value(int64_t op, int64_t padding, double padding_value, bool single
     return op == MC_OP_DILATION ? -std::numeric_limits<double>::infinity() : std::numeric_limits<double>::infinity();
 }
 
+/// mc_dtype of a tensor of the operators that read and write half precision as it is (8-bit activations, the norm).
+int storage_dtype_of(const torch::Tensor& t)
+{
+    switch (t.scalar_type())
+    {
+        case torch::kFloat: return MC_F32;
+        case torch::kDouble: return MC_F64;
+        case torch::kHalf: return MC_F16;
+        case torch::kBFloat16: return MC_BF16;
+        default: TORCH_CHECK(false, "float32, float64, float16 or bfloat16 tensors are expected, got ", t.scalar_type());
+    }
+}
+
+torch::ScalarType scale_type_of(torch::ScalarType t) { return t == torch::kDouble ? torch::kDouble : torch::kFloat; }
+
+int64_t product(c10::IntArrayRef sizes) { return c10::multiply_integers(sizes); }
+
+int64_t code_blocks(int64_t length) { return (length + MC_CODE_BLOCK - 1) / MC_CODE_BLOCK; }
+
+/// A tensor in 8 bits (mc_encode8): codes in its shape, scales [leading dimensions..., blocks of a row]. The rows are what the
+/// dimensions that the scales do not have make up, so that the pair describes itself.
+struct Packed
+{
+    torch::Tensor codes, scales;
+    bool defined() const { return codes.defined(); }
+};
+
+mc_rows_desc rows_desc(const torch::Tensor& t, int64_t leading, int dtype)
+{
+    mc_rows_desc d{};
+    d.rows = product(t.sizes().slice(0, leading));
+    d.length = product(t.sizes().slice(leading));
+    d.dtype = dtype;
+    return d;
+}
+
+Packed encoded(const torch::Tensor& x, int64_t row_dims)
+{
+    const torch::Tensor t = x.contiguous();
+    const int64_t leading = t.dim() - row_dims;
+    const mc_rows_desc d = rows_desc(t, leading, storage_dtype_of(t));
+    std::vector<int64_t> shape = t.sizes().slice(0, leading).vec();
+    shape.push_back(code_blocks(d.length));
+    Packed p{at::empty(t.sizes(), t.options().dtype(torch::kChar)), at::empty(shape, t.options().dtype(scale_type_of(t.scalar_type())))};
+    const TraceRange trace("morphocore::encode8");
+    check_status(mc_encode8(&d, t.data_ptr(), p.codes.data_ptr<int8_t>(), p.scales.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+    return p;
+}
+
+torch::Tensor decoded(const Packed& p, torch::ScalarType dtype)
+{
+    torch::Tensor x = at::empty(p.codes.sizes(), p.codes.options().dtype(dtype));
+    const mc_rows_desc d = rows_desc(x, p.scales.dim() - 1, storage_dtype_of(x));
+    const TraceRange trace("morphocore::decode8");
+    check_status(mc_decode8(&d, p.codes.data_ptr<int8_t>(), p.scales.data_ptr(), x.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+    return x;
+}
+
+/// A pair of tensors that a caller hands over as an activation in 8 bits, checked, contiguous.
+Packed checked_packed(const torch::Tensor& codes, const torch::Tensor& scales)
+{
+    require_cuda(codes, "codes");
+    require_cuda(scales, "scales");
+    TORCH_CHECK(codes.device() == scales.device(), "codes and scales must be on the same device");
+    TORCH_CHECK(codes.scalar_type() == torch::kChar, "codes must be int8, got ", codes.scalar_type());
+    TORCH_CHECK(scales.scalar_type() == torch::kFloat || scales.scalar_type() == torch::kDouble, "scales must be float32 or float64, got ", scales.scalar_type());
+    const int64_t leading = scales.dim() - 1;
+    TORCH_CHECK(leading >= 0 && leading < codes.dim() && scales.sizes().slice(0, leading) == codes.sizes().slice(0, leading)
+                    && scales.size(leading) == code_blocks(product(codes.sizes().slice(leading))),
+                "scales of shape ", scales.sizes(), " do not belong to codes of shape ", codes.sizes());
+    return {codes.contiguous(), scales.contiguous()};
+}
+
+/// How a layer keeps its input for the backward pass.
+struct Keep
+{
+    bool in8 = false;   // in 8 bits, instead of the tensor itself
+    Packed packed;      // already encoded by the caller
+};
+
+/// The 8-bit form of a layer's input: the caller's, or a new one with a row for every plane of pixels (for every image where the
+/// planes have a single pixel, which would need a scale of its own).
+Packed kept_input(const Keep& keep, const torch::Tensor& input4d)
+{
+    if (keep.packed.defined()) return {keep.packed.codes.view(input4d.sizes()), keep.packed.scales};
+    return encoded(input4d, input4d.size(2) * input4d.size(3) == 1 ? 3 : 2);
+}
+
+/// A kept input whose codes were viewed as 4-D: its rows are those of the scales, counted from the front.
+torch::Tensor decoded_input(const torch::Tensor& codes, const torch::Tensor& scales, torch::ScalarType dtype)
+{
+    torch::Tensor x = at::empty(codes.sizes(), codes.options().dtype(dtype));
+    mc_rows_desc d{};
+    d.rows = product(scales.sizes().slice(0, scales.dim() - 1));
+    d.length = d.rows == 0 ? 0 : x.numel() / d.rows;
+    d.dtype = storage_dtype_of(x);
+    const TraceRange trace("morphocore::decode8");
+    check_status(mc_decode8(&d, codes.data_ptr<int8_t>(), scales.data_ptr(), x.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+    return x;
+}
+
+/// What a layer was asked to keep, checked against its input.
+Keep checked_keep(const torch::Tensor& input, const std::optional<torch::Tensor>& codes, const std::optional<torch::Tensor>& scales)
+{
+    Keep keep;
+    keep.in8 = true;
+    const bool given = codes.has_value() && codes->defined();
+    TORCH_CHECK(given == (scales.has_value() && scales->defined()), "codes and scales are given together or not");
+    if (!given) return keep;
+    keep.packed = checked_packed(*codes, *scales);
+    TORCH_CHECK(codes->sizes() == input.sizes(), "the activation in 8 bits has shape ", codes->sizes(), ", the input ", input.sizes());
+    TORCH_CHECK(codes->device() == input.device(), "the activation in 8 bits is on ", codes->device(), ", the input on ", input.device());
+    TORCH_CHECK(scales->scalar_type() == scale_type_of(input.scalar_type()), "the activation in 8 bits was not encoded from a tensor of type ",
+                input.scalar_type());
+    return keep;
+}
+
 /// Whether a call with these inputs goes through the autograd function. Calls that will not be differentiated (inference, or
 /// inputs that need no gradient) skip it, which saves about 2 us of host time, and the winner index of MAX / MIN merges,
 /// whose only reader is the backward pass: on (8, 3, 128, 128) -> 16 channels the search for it took four fifths of the
@@ -177,13 +294,25 @@ class MorphoFunction : public torch::autograd::Function<MorphoFunction>
 {
 public:
     static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor input, torch::Tensor weight, int64_t op, int64_t merge,
-                                 int64_t padding, double padding_value, bool save_indices, double noise_scale, int64_t flags)
+                                 int64_t padding, double padding_value, bool save_indices, double noise_scale, int64_t flags, const Keep& keep)
     {
         MorphoCall call = run_morpho_forward(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags);
         // Erosion's structuring element is saved as a copy (the reference saves the flipped one), so that a program may go on
         // to change the parameter in place before the backward pass.
         if ((flags & MC_FLAG_FLIPPED_WEIGHT) != 0 && call.weight4d.is_alias_of(weight)) call.weight4d = call.weight4d.clone();
-        ctx->save_for_backward({call.input4d, call.weight4d, call.indices, call.sample_weight});
+        // In 8 bits the input is kept as codes, and not at all where the winners are: they are all that the backward pass reads.
+        Packed packed;
+        if (keep.in8 && !call.indices.defined())
+        {
+            const c10::cuda::CUDAGuard device_guard(input.device());
+            packed = kept_input(keep, call.input4d);
+        }
+        if (keep.in8)
+        {
+            ctx->saved_data["sizes"] = call.input4d.sizes().vec();
+            call.input4d = torch::Tensor();
+        }
+        ctx->save_for_backward({call.input4d, call.weight4d, call.indices, call.sample_weight, packed.codes, packed.scales});
         ctx->saved_data["op"] = op;
         ctx->saved_data["merge"] = merge;
         ctx->saved_data["pad_kind"] = static_cast<int64_t>(call.d.pad_kind);
@@ -197,21 +326,22 @@ public:
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grad_outputs)
     {
         const auto saved = ctx->get_saved_variables();
-        const torch::Tensor& input = saved[0];
         const torch::Tensor& weight = saved[1];
         const torch::Tensor& indices = saved[2];
         const torch::Tensor& sample_weight = saved[3];
         torch::Tensor grad_output = input_to_4d(grad_outputs[0]).contiguous();
 
-        std::vector<int64_t> expected = input.sizes().vec();
+        const std::vector<int64_t> input_sizes = saved[0].defined() ? saved[0].sizes().vec() : ctx->saved_data["sizes"].toIntVector();
+        std::vector<int64_t> expected = input_sizes;
         expected[1] = weight.size(0);
         TORCH_CHECK(grad_output.sizes() == c10::IntArrayRef(expected), "grad_output shape mismatch: expected [", c10::IntArrayRef(expected),
                     "] but got [", grad_output.sizes(), "]");
-        TORCH_CHECK(grad_output.device() == input.device(), "grad_output must be on the same device as input");
-        TORCH_CHECK(grad_output.scalar_type() == input.scalar_type(), "grad_output must have the same dtype as input");
+        TORCH_CHECK(grad_output.device() == weight.device(), "grad_output must be on the same device as input");
+        TORCH_CHECK(grad_output.scalar_type() == weight.scalar_type(), "grad_output must have the same dtype as input");
 
-        const c10::cuda::CUDAGuard device_guard(input.device());
-        mc_desc d = make_desc(input, weight, ctx->saved_data["op"].toInt(), ctx->saved_data["merge"].toInt());
+        const c10::cuda::CUDAGuard device_guard(weight.device());
+        torch::Tensor grad_input = torch::empty(input_sizes, weight.options());
+        mc_desc d = make_desc(grad_input, weight, ctx->saved_data["op"].toInt(), ctx->saved_data["merge"].toInt());
         d.pad_kind = static_cast<int32_t>(ctx->saved_data["pad_kind"].toInt());
         d.fill = ctx->saved_data["fill"].toDouble();
         d.flags = static_cast<int32_t>(ctx->saved_data["flags"].toInt());
@@ -219,21 +349,22 @@ public:
         const torch::Tensor& kernel_weight = sample_weight.defined() ? sample_weight : weight;
         if (sample_weight.defined()) d.weight_batch_stride = weight.numel();
 
-        torch::Tensor grad_input = torch::empty_like(input);
         torch::Tensor grad_weight = torch::empty_like(weight);
         const bool have_idx = indices.defined() && indices.numel() > 0;
         const size_t ws_bytes = mc_morpho_backward_workspace_bytes(&d, have_idx);
         torch::Tensor workspace;
-        if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, input.options().dtype(torch::kByte));
+        if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, weight.options().dtype(torch::kByte));
+        const torch::Tensor input = saved[4].defined() ? decoded_input(saved[4], saved[5], weight.scalar_type()) : saved[0];
 
         const TraceRange trace("morphocore::morpho_backward");
-        check_status(mc_morpho_backward(&d, input.data_ptr(), kernel_weight.data_ptr(), have_idx ? indices.data_ptr<int32_t>() : nullptr,
+        check_status(mc_morpho_backward(&d, input.defined() ? input.data_ptr() : nullptr, kernel_weight.data_ptr(), have_idx ? indices.data_ptr<int32_t>() : nullptr,
                                         grad_output.data_ptr(), grad_input.data_ptr(), grad_weight.data_ptr(),
                                         workspace.defined() ? workspace.data_ptr() : nullptr, ws_bytes, at::cuda::getCurrentCUDAStream().stream()));
 
         grad_input = output_to_original(grad_input, ctx->saved_data["input_dims"].toInt());
         if (ctx->saved_data["weight_dims"].toInt() == 2) grad_weight = grad_weight.squeeze(0).squeeze(0);
-        return {grad_input, grad_weight, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+        return {grad_input, grad_weight, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor(),
+                torch::Tensor()};
     }
 };
 
@@ -296,10 +427,17 @@ class MorphoPairFunction : public torch::autograd::Function<MorphoPairFunction>
 {
 public:
     static torch::autograd::tensor_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor input, torch::Tensor weight, int64_t merge,
-                                                int64_t padding, double padding_value)
+                                                int64_t padding, double padding_value, const Keep& keep)
     {
-        const MorphoPairCall call = run_morpho_pair_forward(input, weight, merge, padding, padding_value);
-        ctx->save_for_backward({call.input4d, call.weight4d});
+        MorphoPairCall call = run_morpho_pair_forward(input, weight, merge, padding, padding_value);
+        Packed packed;
+        if (keep.in8)
+        {
+            const c10::cuda::CUDAGuard device_guard(input.device());
+            packed = kept_input(keep, call.input4d);
+            call.input4d = torch::Tensor();
+        }
+        ctx->save_for_backward({call.input4d, call.weight4d, packed.codes, packed.scales});
         ctx->saved_data["merge"] = merge;
         ctx->saved_data["padding"] = padding;
         ctx->saved_data["padding_value"] = padding_value;
@@ -311,11 +449,11 @@ public:
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grad_outputs)
     {
         const auto saved = ctx->get_saved_variables();
-        const torch::Tensor& input = saved[0];
         const torch::Tensor& weight = saved[1];
         const int64_t merge = ctx->saved_data["merge"].toInt(), padding = ctx->saved_data["padding"].toInt();
         const double padding_value = ctx->saved_data["padding_value"].toDouble();
-        const c10::cuda::CUDAGuard device_guard(input.device());
+        const c10::cuda::CUDAGuard device_guard(weight.device());
+        const torch::Tensor input = saved[2].defined() ? decoded_input(saved[2], saved[3], weight.scalar_type()) : saved[0];
         const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
 
         torch::Tensor grad_input, grad_weight;
@@ -352,7 +490,7 @@ public:
             grad_input = output_to_original(grad_input, ctx->saved_data["input_dims"].toInt());
             if (ctx->saved_data["weight_dims"].toInt() == 2) grad_weight = grad_weight.squeeze(0).squeeze(0);
         }
-        return {grad_input, grad_weight, torch::Tensor(), torch::Tensor(), torch::Tensor()};
+        return {grad_input, grad_weight, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
     }
 };
 
@@ -453,36 +591,55 @@ class SmorphFunction : public torch::autograd::Function<SmorphFunction>
 {
 public:
     static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor input, torch::Tensor weight, torch::Tensor alpha, int64_t merge,
-                                 bool reparametrise)
+                                 bool reparametrise, const Keep& keep)
     {
-        const SmorphCall call = run_smorph_forward(input, weight, alpha, merge, reparametrise);
-        // The backward pass reads the 4-D output: the merge target of MAX and MIN.
-        ctx->save_for_backward({call.output, alpha, call.input4d, call.weight4d, call.alphas, save_raw_weight(reparametrise, weight, alpha)});
+        SmorphCall call = run_smorph_forward(input, weight, alpha, merge, reparametrise);
+        // The backward pass reads the 4-D output: the merge target of MAX and MIN. With the input in 8 bits it is that of the kept
+        // input, which the backward pass computes where it needs it.
+        Packed packed;
+        const torch::Tensor result = call.output;
+        if (keep.in8)
+        {
+            const c10::cuda::CUDAGuard device_guard(input.device());
+            packed = kept_input(keep, call.input4d);
+            call.input4d = torch::Tensor();
+            call.output = torch::Tensor();
+        }
+        ctx->save_for_backward({call.output, alpha, call.input4d, call.weight4d, call.alphas, save_raw_weight(reparametrise, weight, alpha),
+                                packed.codes, packed.scales});
         ctx->saved_data["reparametrised"] = reparametrise;
         ctx->saved_data["merge"] = merge;
         ctx->saved_data["input_dims"] = input.dim();
         ctx->saved_data["weight_dims"] = weight.dim();
-        return output_to_original(call.output, input.dim());
+        if (keep.in8) ctx->saved_data["sizes"] = result.sizes().vec();
+        return output_to_original(result, input.dim());
     }
 
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grad_outputs)
     {
         const auto saved = ctx->get_saved_variables();
-        const torch::Tensor& output = saved[0];
         const torch::Tensor& alpha = saved[1];
-        const torch::Tensor& input = saved[2];
         const torch::Tensor& weight = saved[3];
         const torch::Tensor& alphas = saved[4];
         const torch::Tensor& raw_weight = saved[5];
         const int64_t merge = ctx->saved_data["merge"].toInt();
         torch::Tensor grad_output = input_to_4d(grad_outputs[0]).contiguous();
-        TORCH_CHECK(grad_output.sizes() == output.sizes(), "grad_output shape mismatch: expected [", output.sizes(), "] but got [",
-                    grad_output.sizes(), "]");
-        TORCH_CHECK(grad_output.scalar_type() == input.scalar_type(), "grad_output must have the same dtype as input");
-        TORCH_CHECK(grad_output.device() == input.device(), "grad_output must be on the same device as input");
+        const std::vector<int64_t> output_sizes = saved[0].defined() ? saved[0].sizes().vec() : ctx->saved_data["sizes"].toIntVector();
+        TORCH_CHECK(grad_output.sizes() == c10::IntArrayRef(output_sizes), "grad_output shape mismatch: expected [", c10::IntArrayRef(output_sizes),
+                    "] but got [", grad_output.sizes(), "]");
+        TORCH_CHECK(grad_output.scalar_type() == weight.scalar_type(), "grad_output must have the same dtype as input");
+        TORCH_CHECK(grad_output.device() == weight.device(), "grad_output must be on the same device as input");
 
-        const c10::cuda::CUDAGuard device_guard(input.device());
+        const c10::cuda::CUDAGuard device_guard(weight.device());
+        torch::Tensor input = saved[2], output = saved[0];
+        if (saved[6].defined()) input = decoded_input(saved[6], saved[7], weight.scalar_type());
         const mc_desc d = make_desc(input, weight, MC_OP_DILATION, merge);
+        if (saved[6].defined() && (merge == MC_MERGE_MAX || merge == MC_MERGE_MIN))
+        {
+            output = at::empty(output_sizes, weight.options());
+            check_status(mc_smorph_forward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), output.data_ptr(),
+                                           at::cuda::getCurrentCUDAStream().stream()));
+        }
         torch::Tensor grad_input = torch::empty_like(input);
         torch::Tensor grad_weight = torch::empty_like(weight);
         torch::Tensor grad_alpha_pairs = torch::empty_like(alphas);
@@ -492,7 +649,8 @@ public:
 
         const TraceRange trace("morphocore::smorph_backward");
         const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
-        check_status(mc_smorph_backward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), output.data_ptr(), grad_output.data_ptr(),
+        check_status(mc_smorph_backward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), output.defined() ? output.data_ptr() : nullptr,
+                                        grad_output.data_ptr(),
                                         grad_input.data_ptr(), grad_weight.data_ptr(), grad_alpha_pairs.data_ptr(),
                                         workspace.defined() ? workspace.data_ptr() : nullptr, ws_bytes, stream));
         if (ctx->saved_data["reparametrised"].toBool())
@@ -503,7 +661,7 @@ public:
             alpha.numel() == grad_alpha_pairs.numel() ? grad_alpha_pairs.view_as(alpha) : grad_alpha_pairs.sum().view_as(alpha);
         grad_input = output_to_original(grad_input, ctx->saved_data["input_dims"].toInt());
         if (ctx->saved_data["weight_dims"].toInt() == 2) grad_weight = grad_weight.squeeze(0).squeeze(0);
-        return {grad_input, grad_weight, grad_alpha, torch::Tensor(), torch::Tensor()};
+        return {grad_input, grad_weight, grad_alpha, torch::Tensor(), torch::Tensor(), torch::Tensor()};
     }
 };
 
@@ -553,35 +711,53 @@ class SmorphScmFunction : public torch::autograd::Function<SmorphScmFunction>
 {
 public:
     static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor input, torch::Tensor weight, torch::Tensor alpha,
-                                 torch::Tensor beta, bool reparametrise)
+                                 torch::Tensor beta, bool reparametrise, const Keep& keep)
     {
-        const SmorphScmCall call = run_smorph_scm_forward(input, weight, alpha, beta, reparametrise);
-        // The backward pass reads the 4-D output: the final value of the soft merge.
-        ctx->save_for_backward({call.output, alpha, call.betas, call.input4d, call.weight4d, call.alphas, save_raw_weight(reparametrise, weight, alpha)});
+        SmorphScmCall call = run_smorph_scm_forward(input, weight, alpha, beta, reparametrise);
+        // The backward pass reads the 4-D output: the final value of the soft merge, which it computes again for an input in 8 bits.
+        Packed packed;
+        const torch::Tensor result = call.output;
+        if (keep.in8)
+        {
+            const c10::cuda::CUDAGuard device_guard(input.device());
+            packed = kept_input(keep, call.input4d);
+            call.input4d = torch::Tensor();
+            call.output = torch::Tensor();
+        }
+        ctx->save_for_backward({call.output, alpha, call.betas, call.input4d, call.weight4d, call.alphas, save_raw_weight(reparametrise, weight, alpha),
+                                packed.codes, packed.scales});
         ctx->saved_data["reparametrised"] = reparametrise;
         ctx->saved_data["input_dims"] = input.dim();
         ctx->saved_data["weight_dims"] = weight.dim();
-        return output_to_original(call.output, input.dim());
+        if (keep.in8) ctx->saved_data["sizes"] = result.sizes().vec();
+        return output_to_original(result, input.dim());
     }
 
     static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grad_outputs)
     {
         const auto saved = ctx->get_saved_variables();
-        const torch::Tensor& output = saved[0];
         const torch::Tensor& alpha = saved[1];
         const torch::Tensor& beta = saved[2];
-        const torch::Tensor& input = saved[3];
         const torch::Tensor& weight = saved[4];
         const torch::Tensor& alphas = saved[5];
         const torch::Tensor& raw_weight = saved[6];
         torch::Tensor grad_output = input_to_4d(grad_outputs[0]).contiguous();
-        TORCH_CHECK(grad_output.sizes() == output.sizes(), "grad_output shape mismatch: expected [", output.sizes(), "] but got [",
-                    grad_output.sizes(), "]");
-        TORCH_CHECK(grad_output.scalar_type() == input.scalar_type(), "grad_output must have the same dtype as input");
-        TORCH_CHECK(grad_output.device() == input.device(), "grad_output must be on the same device as input");
+        const std::vector<int64_t> output_sizes = saved[0].defined() ? saved[0].sizes().vec() : ctx->saved_data["sizes"].toIntVector();
+        TORCH_CHECK(grad_output.sizes() == c10::IntArrayRef(output_sizes), "grad_output shape mismatch: expected [", c10::IntArrayRef(output_sizes),
+                    "] but got [", grad_output.sizes(), "]");
+        TORCH_CHECK(grad_output.scalar_type() == weight.scalar_type(), "grad_output must have the same dtype as input");
+        TORCH_CHECK(grad_output.device() == weight.device(), "grad_output must be on the same device as input");
 
-        const c10::cuda::CUDAGuard device_guard(input.device());
+        const c10::cuda::CUDAGuard device_guard(weight.device());
+        torch::Tensor input = saved[3], output = saved[0];
+        if (saved[7].defined()) input = decoded_input(saved[7], saved[8], weight.scalar_type());
         const mc_desc d = make_desc(input, weight, MC_OP_DILATION, MC_MERGE_SMOOTH);
+        if (saved[7].defined())
+        {
+            output = at::empty(output_sizes, weight.options());
+            check_status(mc_smorph_scm_forward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), beta.data_ptr(), output.data_ptr(),
+                                               at::cuda::getCurrentCUDAStream().stream()));
+        }
         torch::Tensor grad_input = torch::empty_like(input);
         torch::Tensor grad_weight = torch::empty_like(weight);
         torch::Tensor grad_alpha_pairs = torch::empty_like(alphas);
@@ -601,7 +777,7 @@ public:
             alpha.numel() == grad_alpha_pairs.numel() ? grad_alpha_pairs.view_as(alpha) : grad_alpha_pairs.sum().view_as(alpha);
         grad_input = output_to_original(grad_input, ctx->saved_data["input_dims"].toInt());
         if (ctx->saved_data["weight_dims"].toInt() == 2) grad_weight = grad_weight.squeeze(0).squeeze(0);
-        return {grad_input, grad_weight, grad_alpha, grad_beta, torch::Tensor()};
+        return {grad_input, grad_weight, grad_alpha, grad_beta, torch::Tensor(), torch::Tensor()};
     }
 };
 
@@ -631,9 +807,10 @@ torch::Tensor widen(const torch::Tensor& t, const torch::Tensor& like, const cha
 }
 
 torch::Tensor morpho_call(const torch::Tensor& input, const torch::Tensor& weight, int64_t op, int64_t merge, int64_t padding, double padding_value,
-                          bool save_indices, double noise_scale, int64_t flags = 0)
+                          bool save_indices, double noise_scale, int64_t flags = 0, const Keep& keep = {})
 {
-    if (differentiated({&input, &weight})) return MorphoFunction::apply(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags);
+    if (differentiated({&input, &weight}))
+        return MorphoFunction::apply(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags, keep);
     const at::AutoDispatchBelowADInplaceOrView guard;
     return output_to_original(run_morpho_forward(input, weight, op, merge, padding, padding_value, false, noise_scale, flags).output, input.dim());
 }
@@ -666,42 +843,49 @@ torch::Tensor erosion_layer(torch::Tensor input, torch::Tensor weight, int64_t m
     return morpho_call(input, weight, MC_OP_EROSION, checked_merge(merge), checked_padding(padding), padding_value, save_indices, 0.0, MC_FLAG_FLIPPED_WEIGHT);
 }
 
-/// Extension (not an operator of the reference): both halves of sigma_layer at once. MAX / MIN merges that keep their
-/// winner indices for the backward pass run the two separate operators, which is what saves them.
-std::tuple<torch::Tensor, torch::Tensor> dilation_erosion(torch::Tensor input, torch::Tensor weight, int64_t merge, int64_t padding, double padding_value,
-                                                          bool save_indices)
+std::tuple<torch::Tensor, torch::Tensor> pair_call(const torch::Tensor& input, const torch::Tensor& weight, int64_t merge, int64_t padding,
+                                                   double padding_value, bool save_indices, const Keep& keep = {})
 {
     if (is_reduced(input))
     {
-        auto [d, e] = dilation_erosion(input.to(torch::kFloat), widen(weight, input, "weight"), merge, padding, padding_value, save_indices);
+        auto [d, e] = pair_call(input.to(torch::kFloat), widen(weight, input, "weight"), merge, padding, padding_value, save_indices, keep);
         return {d.to(input.scalar_type()), e.to(input.scalar_type())};
     }
     merge = checked_merge(merge);
     padding = checked_padding(padding);
     if (save_indices && (merge == MC_MERGE_MAX || merge == MC_MERGE_MIN) && differentiated({&input, &weight}))
-        return {dilation(input, weight, merge, padding, padding_value, true, 0.0),
-                erosion_layer(input, weight, merge, padding, padding_value, true)};
+        return {morpho_call(input, weight, MC_OP_DILATION, merge, padding, padding_value, true, 0.0, 0, keep),
+                morpho_call(input, weight, MC_OP_EROSION, merge, padding, padding_value, true, 0.0, MC_FLAG_FLIPPED_WEIGHT, keep)};
     if (!differentiated({&input, &weight}))
     {
         const at::AutoDispatchBelowADInplaceOrView guard;
         const MorphoPairCall call = run_morpho_pair_forward(input, weight, merge, padding, padding_value);
         return {output_to_original(call.out_dilation, input.dim()), output_to_original(call.out_erosion, input.dim())};
     }
-    const auto out = MorphoPairFunction::apply(input, weight, merge, padding, padding_value);
+    const auto out = MorphoPairFunction::apply(input, weight, merge, padding, padding_value, keep);
     return {out[0], out[1]};
 }
 
-torch::Tensor smorph_call(const torch::Tensor& input, const torch::Tensor& weight, const torch::Tensor& alpha, int64_t merge, bool reparametrise)
+/// Extension (not an operator of the reference): both halves of sigma_layer at once. MAX / MIN merges that keep their
+/// winner indices for the backward pass run the two separate operators, which is what saves them.
+std::tuple<torch::Tensor, torch::Tensor> dilation_erosion(torch::Tensor input, torch::Tensor weight, int64_t merge, int64_t padding, double padding_value,
+                                                          bool save_indices)
 {
-    if (differentiated({&input, &weight, &alpha})) return SmorphFunction::apply(input, weight, alpha, merge, reparametrise);
+    return pair_call(input, weight, merge, padding, padding_value, save_indices);
+}
+
+torch::Tensor smorph_call(const torch::Tensor& input, const torch::Tensor& weight, const torch::Tensor& alpha, int64_t merge, bool reparametrise,
+                          const Keep& keep = {})
+{
+    if (differentiated({&input, &weight, &alpha})) return SmorphFunction::apply(input, weight, alpha, merge, reparametrise, keep);
     const at::AutoDispatchBelowADInplaceOrView guard;
     return output_to_original(run_smorph_forward(input, weight, alpha, merge, reparametrise).output, input.dim());
 }
 
 torch::Tensor smorph_scm_call(const torch::Tensor& input, const torch::Tensor& weight, const torch::Tensor& alpha, const torch::Tensor& beta,
-                              bool reparametrise)
+                              bool reparametrise, const Keep& keep = {})
 {
-    if (differentiated({&input, &weight, &alpha, &beta})) return SmorphScmFunction::apply(input, weight, alpha, beta, reparametrise);
+    if (differentiated({&input, &weight, &alpha, &beta})) return SmorphScmFunction::apply(input, weight, alpha, beta, reparametrise, keep);
     const at::AutoDispatchBelowADInplaceOrView guard;
     return output_to_original(run_smorph_scm_forward(input, weight, alpha, beta, reparametrise).output, input.dim());
 }
@@ -745,7 +929,8 @@ bool kernel_reparametrises(const torch::Tensor& input, const torch::Tensor& weig
 /// element (morphocore/functional/smorph.py:60-68) included. As a chain of tensor operations that is ten launches forward
 /// and eighteen backward, 80 and 150 us of host time around kernels that take 20 us on small feature maps; here it is one
 /// launch each way. `beta` selects the smooth channel merge; `merge` IDENTITY then only says how alpha is shaped.
-torch::Tensor smorph_layer(torch::Tensor input, torch::Tensor weight, torch::Tensor alpha, const std::optional<torch::Tensor>& beta, int64_t merge)
+torch::Tensor smorph_layer_call(const torch::Tensor& input, const torch::Tensor& weight, const torch::Tensor& alpha, const std::optional<torch::Tensor>& beta,
+                                int64_t merge, const Keep& keep = {})
 {
     const bool smooth = beta.has_value() && beta->defined();
     checked_smorph_merge(merge);
@@ -753,16 +938,217 @@ torch::Tensor smorph_layer(torch::Tensor input, torch::Tensor weight, torch::Ten
     {
         std::optional<torch::Tensor> wide_beta;
         if (smooth) wide_beta = widen(*beta, input, "beta");
-        return smorph_layer(input.to(torch::kFloat), widen(weight, input, "weight"), widen(alpha, input, "alpha"), wide_beta, merge)
+        return smorph_layer_call(input.to(torch::kFloat), widen(weight, input, "weight"), widen(alpha, input, "alpha"), wide_beta, merge, keep)
             .to(input.scalar_type());
     }
     const bool identity = merge == MC_MERGE_IDENTITY;
     if (kernel_reparametrises(input, weight, alpha, identity, smooth))
-        return smooth ? smorph_scm_call(input, weight, alpha, *beta, true) : smorph_call(input, weight, alpha, merge, true);
+        return smooth ? smorph_scm_call(input, weight, alpha, *beta, true, keep) : smorph_call(input, weight, alpha, merge, true, keep);
     torch::Tensor t = torch::tanh(alpha);
     t = identity || alpha.dim() == 1 ? t.view({-1, 1, 1, 1}) : t.unsqueeze(-1).unsqueeze(-1);
     const torch::Tensor tilde = t * ((1 - t) / 2 * weight.flip({-2, -1}) + (1 + t) / 2 * weight);
-    return smooth ? smorph_scm(input, tilde, alpha, *beta) : smorph(input, tilde, alpha, merge);
+    return smooth ? smorph_scm_call(input, tilde, alpha, *beta, false, keep) : smorph_call(input, tilde, alpha, merge, false, keep);
+}
+
+torch::Tensor smorph_layer(torch::Tensor input, torch::Tensor weight, torch::Tensor alpha, const std::optional<torch::Tensor>& beta, int64_t merge)
+{
+    return smorph_layer_call(input, weight, alpha, beta, merge);
+}
+
+/// Extensions (not operators of the reference): the layers with their input kept in 8 bits for the backward pass, whose
+/// gradients are those at the values that the codes stand for. `codes` and `scales`, where the caller has them already (a norm
+/// with an 8-bit output in front of the layer), are those of `input`; otherwise the operator encodes it. MAX / MIN merges of
+/// dilation and erosion that save their winning indices keep those, and no input.
+torch::Tensor morpho_8bit(torch::Tensor input, torch::Tensor weight, const std::optional<torch::Tensor>& codes, const std::optional<torch::Tensor>& scales,
+                          int64_t op, int64_t merge, int64_t padding, double padding_value, bool save_indices, double noise_scale, bool flipped)
+{
+    TORCH_CHECK(op == MC_OP_DILATION || op == MC_OP_EROSION, "unknown operation ", op);
+    const Keep keep = checked_keep(input, codes, scales);
+    const int64_t flags = flipped ? MC_FLAG_FLIPPED_WEIGHT : 0;
+    merge = checked_merge(merge);
+    padding = checked_padding(padding);
+    if (is_reduced(input))
+        return morpho_call(input.to(torch::kFloat), widen(weight, input, "weight"), op, merge, padding, padding_value, save_indices, noise_scale, flags, keep)
+            .to(input.scalar_type());
+    return morpho_call(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags, keep);
+}
+
+std::tuple<torch::Tensor, torch::Tensor> dilation_erosion_8bit(torch::Tensor input, torch::Tensor weight, const std::optional<torch::Tensor>& codes,
+                                                               const std::optional<torch::Tensor>& scales, int64_t merge, int64_t padding,
+                                                               double padding_value, bool save_indices)
+{
+    return pair_call(input, weight, merge, padding, padding_value, save_indices, checked_keep(input, codes, scales));
+}
+
+torch::Tensor smorph_8bit(torch::Tensor input, torch::Tensor weight, torch::Tensor alpha, const std::optional<torch::Tensor>& beta,
+                          const std::optional<torch::Tensor>& codes, const std::optional<torch::Tensor>& scales, int64_t merge)
+{
+    return smorph_layer_call(input, weight, alpha, beta, merge, checked_keep(input, codes, scales));
+}
+
+/// Extension: the 8-bit form of a tensor. `row_dims` trailing dimensions make up a row, the last block of which may be short.
+std::tuple<torch::Tensor, torch::Tensor> encode_8bit(torch::Tensor input, int64_t row_dims)
+{
+    require_cuda(input, "input");
+    TORCH_CHECK(input.dim() >= 1, "a tensor of one dimension or more is expected");
+    TORCH_CHECK(row_dims >= 1 && row_dims <= input.dim(), "row_dims must be between 1 and the input's ", input.dim(), " dimensions, got ", row_dims);
+    storage_dtype_of(input);
+    const c10::cuda::CUDAGuard device_guard(input.device());
+    const at::AutoDispatchBelowADInplaceOrView guard;   // whole numbers: no gradient flows
+    const Packed p = encoded(input, row_dims);
+    return {p.codes, p.scales};
+}
+
+torch::Tensor decode_8bit(torch::Tensor codes, torch::Tensor scales, torch::ScalarType dtype)
+{
+    const Packed p = checked_packed(codes, scales);
+    TORCH_CHECK(scale_type_of(dtype) == scales.scalar_type(), "scales of type ", scales.scalar_type(), " do not decode to ", dtype);
+    const c10::cuda::CUDAGuard device_guard(codes.device());
+    return decoded(p, dtype);
+}
+
+/// One root-mean-square norm: its shape as [outer, channels, inner], and what came of it.
+struct NormCall
+{
+    mc_norm_desc d{};
+    torch::Tensor x, residual, weight;   // contiguous; the last two may be undefined
+    torch::Tensor sum, y;
+    Packed y_packed, sum_packed;
+};
+
+NormCall run_rms_norm(const torch::Tensor& x, const torch::Tensor& residual, const torch::Tensor& weight, double eps, int64_t dim, bool want_y, bool want_codes,
+                      bool keep8)
+{
+    require_cuda(x, "x");
+    const int dtype = storage_dtype_of(x);
+    TORCH_CHECK(dim >= -x.dim() && dim < x.dim(), "x has ", x.dim(), " dimensions and none numbered ", dim);
+    if (dim < 0) dim += x.dim();
+    TORCH_CHECK(x.size(dim) > 0, "a norm over no channels");
+    TORCH_CHECK(want_y || want_codes, "nothing to compute");
+    if (residual.defined())
+    {
+        TORCH_CHECK(residual.sizes() == x.sizes(), "residual has shape ", residual.sizes(), ", x ", x.sizes());
+        TORCH_CHECK(residual.device() == x.device(), "residual is on ", residual.device(), ", x on ", x.device());
+        TORCH_CHECK(residual.scalar_type() == x.scalar_type(), "residual must have the type of x (", x.scalar_type(), "), got ", residual.scalar_type());
+    }
+    if (weight.defined())
+    {
+        TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(dim), "weight must have shape [", x.size(dim), "], got ", weight.sizes());
+        TORCH_CHECK(weight.device() == x.device(), "weight is on ", weight.device(), ", x on ", x.device());
+        TORCH_CHECK(weight.scalar_type() == x.scalar_type(), "weight must have the type of x (", x.scalar_type(), "), got ", weight.scalar_type());
+    }
+    const c10::cuda::CUDAGuard device_guard(x.device());
+    NormCall call;
+    call.x = x.contiguous();
+    if (residual.defined()) call.residual = residual.contiguous();
+    if (weight.defined()) call.weight = weight.contiguous();
+    call.d.outer = product(x.sizes().slice(0, dim));
+    call.d.channels = x.size(dim);
+    call.d.inner = product(x.sizes().slice(dim + 1));
+    call.d.eps = eps;
+    call.d.dtype = dtype;
+    const auto packed_like_x = [&]() -> Packed {
+        std::vector<int64_t> shape = x.sizes().slice(0, call.d.inner == 1 ? dim : dim + 1).vec();
+        shape.push_back(code_blocks(call.d.inner == 1 ? call.d.channels : call.d.inner));
+        return {at::empty(x.sizes(), call.x.options().dtype(torch::kChar)), at::empty(shape, call.x.options().dtype(scale_type_of(x.scalar_type())))};
+    };
+    if (residual.defined()) call.sum = at::empty(x.sizes(), call.x.options());
+    if (want_y) call.y = at::empty(x.sizes(), call.x.options());
+    if (want_codes) call.y_packed = packed_like_x();
+    if (keep8) call.sum_packed = packed_like_x();
+    const auto data = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+    const auto codes = [](const Packed& p) { return p.defined() ? p.codes.data_ptr<int8_t>() : nullptr; };
+    const TraceRange trace("morphocore::rms_norm_forward");
+    check_status(mc_rms_norm_forward(&call.d, call.x.data_ptr(), data(call.residual), data(call.weight), data(call.sum), data(call.y), codes(call.y_packed),
+                                     data(call.y_packed.scales), codes(call.sum_packed), data(call.sum_packed.scales),
+                                     at::cuda::getCurrentCUDAStream().stream()));
+    return call;
+}
+
+/// y, sum, codes and scales of the call, those that it has.
+torch::autograd::tensor_list norm_outputs(const NormCall& call)
+{
+    torch::autograd::tensor_list out;
+    for (const torch::Tensor& t : {call.y, call.sum, call.y_packed.codes, call.y_packed.scales})
+        if (t.defined()) out.push_back(t);
+    return out;
+}
+
+/// The norm with its gradients. What the backward pass keeps is the sum (x where there is no residual), or its 8-bit form.
+class RmsNormFunction : public torch::autograd::Function<RmsNormFunction>
+{
+public:
+    static torch::autograd::tensor_list forward(torch::autograd::AutogradContext* ctx, torch::Tensor x, const std::optional<torch::Tensor>& with_residual,
+                                                const std::optional<torch::Tensor>& with_weight, double eps, int64_t dim, bool want_codes, bool keep8)
+    {
+        const torch::Tensor residual = with_residual.value_or(torch::Tensor()), weight = with_weight.value_or(torch::Tensor());
+        const NormCall call = run_rms_norm(x, residual, weight, eps, dim, true, want_codes, keep8);
+        const torch::Tensor kept = keep8 ? torch::Tensor() : residual.defined() ? call.sum : call.x;
+        ctx->save_for_backward({kept, call.sum_packed.codes, call.sum_packed.scales, call.weight});
+        ctx->set_materialize_grads(false);
+        ctx->saved_data["sizes"] = c10::IntArrayRef({call.d.outer, call.d.channels, call.d.inner}).vec();
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["residual"] = residual.defined();
+        if (want_codes) ctx->mark_non_differentiable({call.y_packed.codes, call.y_packed.scales});
+        return norm_outputs(call);
+    }
+
+    static torch::autograd::tensor_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::tensor_list grad_outputs)
+    {
+        TORCH_CHECK(!at::GradMode::is_enabled(), "rms_norm is differentiable once: create_graph is not supported");
+        const auto saved = ctx->get_saved_variables();
+        const torch::Tensor &kept = saved[0], &codes = saved[1], &scales = saved[2], &weight = saved[3];
+        const bool residual = ctx->saved_data["residual"].toBool();
+        const torch::Tensor gy = grad_outputs[0].defined() ? grad_outputs[0].contiguous() : torch::Tensor();
+        const torch::Tensor gsum = residual && grad_outputs[1].defined() ? grad_outputs[1].contiguous() : torch::Tensor();
+        torch::Tensor gx, gweight;
+        const torch::Tensor& like = gy.defined() ? gy : gsum;
+        if (like.defined())
+        {
+            const c10::cuda::CUDAGuard device_guard(like.device());
+            if (weight.defined()) gweight = at::empty_like(weight);
+            if (!gy.defined())   // the norm itself was not used
+            {
+                gx = gsum;
+                if (weight.defined()) gweight.zero_();
+            }
+            else
+            {
+                const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+                mc_norm_desc d{};
+                d.outer = sizes[0];
+                d.channels = sizes[1];
+                d.inner = sizes[2];
+                d.eps = ctx->saved_data["eps"].toDouble();
+                d.dtype = storage_dtype_of(gy);
+                gx = at::empty_like(gy);
+                const size_t ws_bytes = mc_rms_norm_backward_workspace_bytes(&d, weight.defined());
+                torch::Tensor workspace;
+                if (ws_bytes > 0) workspace = at::empty({static_cast<int64_t>(ws_bytes)}, gy.options().dtype(torch::kByte));
+                const auto data = [](const torch::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+                const TraceRange trace("morphocore::rms_norm_backward");
+                check_status(mc_rms_norm_backward(&d, data(kept), codes.defined() ? codes.data_ptr<int8_t>() : nullptr, data(scales), data(weight),
+                                                  gy.data_ptr(), data(gsum), gx.data_ptr(), data(gweight), data(workspace), ws_bytes,
+                                                  at::cuda::getCurrentCUDAStream().stream()));
+            }
+        }
+        return {gx, residual ? gx : torch::Tensor(), gweight, torch::Tensor(), torch::Tensor(), torch::Tensor(), torch::Tensor()};
+    }
+};
+
+/// Extension: root-mean-square norm along `dim`, after the addition of a residual. Returns, of y, the sum, codes and scales, those
+/// that were asked for; `keep8` keeps what the backward pass reads in 8 bits.
+std::vector<torch::Tensor> rms_norm(torch::Tensor x, const std::optional<torch::Tensor>& residual, const std::optional<torch::Tensor>& weight, double eps,
+                                    int64_t dim, bool want_y, bool want_codes, bool keep8)
+{
+    const torch::Tensor r = residual.value_or(torch::Tensor()), w = weight.value_or(torch::Tensor());
+    if (differentiated({&x, r.defined() ? &r : &x, w.defined() ? &w : &x}))
+    {
+        TORCH_CHECK(want_y, "an output in 8 bits alone has no gradient: ask for both, or call under torch.no_grad()");
+        return RmsNormFunction::apply(x, residual, weight, eps, dim, want_codes, keep8);
+    }
+    const at::AutoDispatchBelowADInplaceOrView guard;
+    return norm_outputs(run_rms_norm(x, r, w, eps, dim, want_y, want_codes, false));
 }
 
 }  // namespace
@@ -778,6 +1164,14 @@ TORCH_LIBRARY(morphocore, m)
     m.def("dilation_erosion(Tensor input, Tensor weight, int merge, int padding, float padding_value=0., bool save_indices=True) -> (Tensor, Tensor)");
     m.def("smorph_layer(Tensor input, Tensor weight, Tensor alpha, Tensor? beta, int merge) -> Tensor");
     m.def("erosion_layer(Tensor input, Tensor weight, int merge, int padding, float padding_value=0., bool save_indices=True) -> Tensor");
+    m.def("morpho_8bit(Tensor input, Tensor weight, Tensor? codes, Tensor? scales, int op, int merge, int padding, float padding_value=0., "
+          "bool save_indices=True, float noise_scale=0., bool flipped=False) -> Tensor");
+    m.def("dilation_erosion_8bit(Tensor input, Tensor weight, Tensor? codes, Tensor? scales, int merge, int padding, float padding_value=0., "
+          "bool save_indices=True) -> (Tensor, Tensor)");
+    m.def("smorph_8bit(Tensor input, Tensor weight, Tensor alpha, Tensor? beta, Tensor? codes, Tensor? scales, int merge) -> Tensor");
+    m.def("encode_8bit(Tensor input, int row_dims=2) -> (Tensor, Tensor)");
+    m.def("decode_8bit(Tensor codes, Tensor scales, ScalarType dtype) -> Tensor");
+    m.def("rms_norm(Tensor x, Tensor? residual, Tensor? weight, float eps, int dim, bool want_y=True, bool want_codes=False, bool keep8=False) -> Tensor[]");
 }
 
 TORCH_LIBRARY_IMPL(morphocore, CompositeImplicitAutograd, m)
@@ -789,4 +1183,10 @@ TORCH_LIBRARY_IMPL(morphocore, CompositeImplicitAutograd, m)
     m.impl("dilation_erosion", &dilation_erosion);
     m.impl("smorph_layer", &smorph_layer);
     m.impl("erosion_layer", &erosion_layer);
+    m.impl("morpho_8bit", &morpho_8bit);
+    m.impl("dilation_erosion_8bit", &dilation_erosion_8bit);
+    m.impl("smorph_8bit", &smorph_8bit);
+    m.impl("encode_8bit", &encode_8bit);
+    m.impl("decode_8bit", &decode_8bit);
+    m.impl("rms_norm", &rms_norm);
 }

@@ -3,6 +3,7 @@
 import torch
 
 from ._ops import ops
+from .activation8 import keeping_8bit, kept_codes
 from .dilation import dilation
 from .erosion import erosion
 from .merge_enum import str_to_merge, str_to_padding
@@ -35,8 +36,11 @@ def sigma_layer(x: torch.Tensor, w: torch.Tensor, alpha: torch.Tensor, channel_m
     if not (training and (weight_dropout > 0.0 or noise_scale > 0.0)):
         # Both stages see the same structuring element: one operator computes the two (a single fused pass over x where the
         # kernel covers the case, the two separate passes otherwise; same values either way).
-        out_dilation, out_erosion = ops.dilation_erosion(x, w, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
-                                                         padding_value, save_indices)
+        modes = str_to_merge(channel_merge_mode), str_to_padding(padding_mode), padding_value, save_indices
+        if keeping_8bit():
+            out_dilation, out_erosion = ops.dilation_erosion_8bit(x, w, *kept_codes(), *modes)
+        else:
+            out_dilation, out_erosion = ops.dilation_erosion(x, w, *modes)
     else:
         # Each stage draws its own dropout mask and noise (morphocore/functional/sigma_layer.py:73-78).
         kwargs = dict(channel_merge_mode=channel_merge_mode, padding_mode=padding_mode, save_indices=save_indices,
@@ -45,3 +49,6 @@ def sigma_layer(x: torch.Tensor, w: torch.Tensor, alpha: torch.Tensor, channel_m
         out_dilation = dilation(x, w, **kwargs)
     soft = torch.sigmoid(alpha.mean(dim=1)).view(1, -1, 1, 1)
     return out_erosion * (1.0 - soft) + out_dilation * soft
+
+
+sigma_layer.takes_packed = True

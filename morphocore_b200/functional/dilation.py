@@ -2,6 +2,7 @@ import torch
 
 from ._dropout import drop_weights
 from ._ops import ops
+from .activation8 import keeping_8bit, kept_codes
 from .merge_enum import str_to_merge, str_to_padding
 
 
@@ -29,5 +30,11 @@ def dilation(x: torch.Tensor, w: torch.Tensor, channel_merge_mode: str = 'sum',
     """
     if training and weight_dropout > 0.0:
         w = drop_weights(w, weight_dropout)
+    if keeping_8bit():
+        return ops.morpho_8bit(x, w, *kept_codes(), 0, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
+                               padding_value, save_indices, noise_scale if training else 0.0)
     return ops.dilation(x, w, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
                         padding_value, save_indices, noise_scale if training else 0.0)
+
+
+dilation.takes_packed = True

@@ -2,6 +2,7 @@ import torch
 
 from ._dropout import drop_weights
 from ._ops import ops
+from .activation8 import keeping_8bit, kept_codes
 from .merge_enum import str_to_merge, str_to_padding
 
 
@@ -21,8 +22,15 @@ def erosion(x: torch.Tensor, w: torch.Tensor, channel_merge_mode: str = 'sum',
     """
     if training and weight_dropout > 0.0:
         w = drop_weights(w, weight_dropout)
-    if not training or noise_scale == 0.0:
+    noisy = training and noise_scale != 0.0
+    if keeping_8bit():
+        return ops.morpho_8bit(x, w.flip((-2, -1)) if noisy else w, *kept_codes(), 1, str_to_merge(channel_merge_mode),
+                               str_to_padding(padding_mode), padding_value, save_indices, noise_scale if noisy else 0.0, not noisy)
+    if not noisy:
         return ops.erosion_layer(x, w, str_to_merge(channel_merge_mode), str_to_padding(padding_mode), padding_value, save_indices)
     # The per-sample noise is drawn for the flipped structuring element.
     return ops.erosion(x, w.flip((-2, -1)), str_to_merge(channel_merge_mode),
                        str_to_padding(padding_mode), padding_value, save_indices, noise_scale)
+
+
+erosion.takes_packed = True

@@ -1,6 +1,7 @@
 import torch
 
 from ._ops import ops
+from .activation8 import keeping_8bit, kept_codes
 from .merge_enum import MorphoMerge, str_to_merge
 
 
@@ -29,4 +30,9 @@ def smorph(x: torch.Tensor, w: torch.Tensor, alpha: torch.Tensor, beta: torch.Te
         merge = MorphoMerge.IDENTITY if channel_merge_mode == 'identity' else MorphoMerge.ADD
     else:
         merge = str_to_merge(channel_merge_mode)
+    if keeping_8bit():
+        return ops.smorph_8bit(x, w, alpha, beta, *kept_codes(), merge)
     return ops.smorph_layer(x, w, alpha, beta, merge)
+
+
+smorph.takes_packed = True

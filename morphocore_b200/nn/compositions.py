@@ -63,6 +63,7 @@ class Closing(_TwoStage):
 
 class SigmaLayer(AlphaModule):
     """Learnable blend sigmoid(alpha) * dilation + (1 - sigmoid(alpha)) * erosion with one structuring element."""
+    takes_packed = True   # checkpoint_8bit may be given the 8-bit form of the input
 
     def __init__(self, in_channels: int, out_channels: int, kernel_size: tuple, channel_merge_mode: str = "sum",
                  padding_mode: str = "replicate", init_alpha: float = 0.0, dtype: torch.dtype = torch.float32,

@@ -9,6 +9,8 @@ class Erosion(MorphoModule):
     reference `morphocore.nn.Erosion` (morphocore/nn/erosion.py:86-101). See
     `morphocore_b200.functional.erosion` for the arguments."""
 
+    takes_packed = True   # checkpoint_8bit may be given the 8-bit form of the input
+
     def __init__(self, in_channels: int, out_channels: int, kernel_size: tuple,
                  channel_merge_mode: str = "sum", padding_mode: str = "replicate",
                  dtype: torch.dtype = torch.float32, save_indices: bool = True,

@@ -13,6 +13,8 @@ class SMorph(AlphaModule):
     channel (morphocore/functional/csrc/cpp/smorph_scm.cpp:31), so, as in the reference, the forward
     pass of such a module raises unless in_channels == 1. functional.smorph takes a (out_channels,) beta."""
 
+    takes_packed = True   # checkpoint_8bit may be given the 8-bit form of the input
+
     def __init__(self, in_channels: int, out_channels: int, kernel_size: tuple, channel_merge_mode: str = "sum",
                  init_alpha: float = 0.0, dtype: torch.dtype = torch.float32, init_beta: float = None):
         if type(kernel_size) is int:

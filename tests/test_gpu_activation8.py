@@ -1,0 +1,417 @@
+"""8-bit activations on the GPU, and the layers that keep their input in them, against plain implementations in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import _plain8 as P
+import morphocore_b200.functional as F
+import morphocore_b200.nn as Mnn
+from oracle import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.bfloat16, torch.float16, torch.float64]
+SHAPES = [((1,), 1), ((3, 2), 1), ((2, 3, 1, 1), 2), ((5, 127), 1), ((2, 128), 1), ((3, 129), 1), ((1, 260), 1), ((7, 8192), 1), ((2, 3, 7, 7), 2),
+          ((3, 5, 12, 20), 2), ((2, 2, 75, 101), 2), ((2, 3, 4, 5), 4), ((700, 3), 1), ((0, 4), 1), ((2, 0, 4, 4), 2), ((2, 3, 0, 4), 2)]
+
+
+def make(shape, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g, dtype=torch.float64) * 3).to(dtype)
+
+
+def same(a, b):
+    """Equal, NaN included."""
+    return a.shape == b.shape and bool(((a == b) | ((a != a) & (b != b))).all())
+
+
+def check(x, row_dims, device_x=None):
+    """Codes and scales bit for bit, and the decoded values: a code is a whole number, so there is nothing to tolerate but in
+    double, where the plain product is rounded to 64 bits of mantissa before it is rounded to a whole number."""
+    packed = F.encode_8bit(x.cuda() if device_x is None else device_x, row_dims)
+    codes, scales, _ = P.encode(x, row_dims)
+    assert packed.dtype == x.dtype and packed.codes.dtype == torch.int8
+    assert packed.scales.dtype == (torch.float64 if x.dtype == torch.float64 else torch.float32)
+    assert np.array_equal(packed.scales.cpu().numpy(), scales)
+    assert np.array_equal(packed.codes.cpu().numpy(), codes)
+    values = F.decode_8bit(packed)
+    assert values.dtype == x.dtype
+    assert same(values.cpu(), P.decode(torch.from_numpy(codes), torch.from_numpy(scales), x.dtype))
+    return packed, values
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,row_dims", SHAPES, ids=str)
+def test_codes(shape, row_dims, dtype):
+    x = make(shape, dtype)
+    packed, values = check(x, row_dims)
+    if not x.numel():
+        return
+    # Half a scale, its own rounding and that of the product (three half steps of values up to 126 scales), and the type's.
+    rows, length, _ = P.rows_of(shape, row_dims)
+    u = torch.finfo(packed.scales.dtype).eps / 2
+    scale = packed.scales.cpu().double().reshape(rows, -1).repeat_interleave(P.BLOCK, 1)[:, :length].reshape(shape)
+    bound = scale * (0.5 + 3 * 126 * u) + values.cpu().double().abs() * torch.finfo(dtype).eps / 2
+    assert bool(((values.cpu().double() - x.double()).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("length", [128, 131, 300])
+def test_values_without_a_number(dtype, length):
+    """Infinities and NaN come back as they are and leave the rest of their block alone; blocks of nothing else, of zeros, of the type's
+    lowest value, of its largest, and of magnitudes too small for a scale."""
+    x = make((12, length), dtype, 1)
+    inf, nan, info = float("inf"), float("nan"), torch.finfo(dtype)
+    x[0, 3], x[0, 64], x[0, 100] = inf, -inf, nan
+    x[1, ::2] = -inf
+    x[2] = nan
+    x[3] = -inf
+    x[4] = 0
+    x[5] = info.min
+    x[6, 5], x[6, 6] = info.max, info.min
+    x[7] *= 2.0 ** -100 if dtype != torch.float64 else 2.0 ** -900
+    x[8] = info.tiny
+    x[9] = info.smallest_normal * 0.25
+    x[10, :127] = 0
+    x[11] = -0.0
+    packed, values = check(x, 1)
+    plain = x.double()
+    assert bool((values.isnan().cpu() == x.isnan()).all()) and bool((values.isinf().cpu() == x.isinf()).all())
+    assert bool((values[4] == 0).all()) and bool((values[11] == 0).all())
+    if dtype in (torch.float32, torch.float64):
+        assert not packed.scales[8].any() and not packed.scales[9].any()
+    # The finite ones beside the infinities: half a scale, top / 252, with the roundings of 126 / m, of the scale and of its product
+    # with a code (three half steps of top at most), and half a step of the tensor's type, of top or less.
+    top = float(plain[1, 1::2].abs().max())
+    u = torch.finfo(torch.float64 if dtype == torch.float64 else torch.float32).eps / 2
+    off = (values[1, 1::2].cpu().double() - plain[1, 1::2]).abs().max()
+    assert bool((values[1, ::2] == -inf).all()) and float(off) <= top * (1 / 252 + 3 * u + info.eps / 2)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_layouts_and_alignment(dtype):
+    """Views that start off the boundary of a wide load, strided, broadcast and permuted tensors, and a sliced 8-bit form."""
+    flat = make((4 * 6 * 128 + 7,), dtype, 2)
+    for offset in (0, 1, 2, 3, 4):
+        x = flat[offset:offset + 4 * 6 * 128].view(4, 6, 128)
+        check(x, 1, flat.cuda()[offset:offset + 4 * 6 * 128].view(4, 6, 128))
+    x = make((3, 4, 6, 10), dtype, 3)
+    for view in (lambda t: t.permute(0, 2, 3, 1), lambda t: t[:, ::2, 1:, ::3], lambda t: t[:1].expand(5, 4, 6, 10), lambda t: t.transpose(0, 3),
+                 lambda t: t.to(memory_format=torch.channels_last)):
+        check(view(x).contiguous(), 2, view(x.cuda()))
+    packed, values = check(x, 2)
+    assert same(F.decode_8bit(F.Activation8(packed.codes[1:], packed.scales[1:], dtype)), values[1:])
+    assert same(F.decode_8bit(F.Activation8(packed.codes[:, ::2], packed.scales[:, ::2], dtype)), values[:, ::2])
+
+
+def test_long_tensors():
+    """More than 2^31 elements: the last rows are those of a tensor of their own."""
+    length, rows = 128 * 1024 + 64, 16500
+    assert length * rows > 2 ** 31
+    x = torch.empty(rows, length, dtype=torch.bfloat16, device="cuda")
+    x[:-2] = 1.0
+    x[-2:] = make((2, length), torch.bfloat16, 4).cuda()
+    packed = F.encode_8bit(x, 1)
+    tail = F.encode_8bit(x[-2:], 1)
+    assert bool((packed.codes[-2:] == tail.codes).all()) and bool((packed.scales[-2:] == tail.scales).all())
+    assert bool((packed.codes[:-2:611] == 126).all())
+    values = F.decode_8bit(packed)
+    assert bool((values[-2:] == F.decode_8bit(tail)).all()) and bool((values[::997][:-1] == 1).all())
+
+
+def test_streams_and_graphs():
+    x = make((6, 10, 33, 35), torch.float32, 5).cuda()
+    want = F.encode_8bit(x)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = F.encode_8bit(x)
+        values = F.decode_8bit(got)
+    torch.cuda.current_stream().wait_stream(side)
+    assert bool((got.codes == want.codes).all()) and bool((got.scales == want.scales).all()) and bool((values == F.decode_8bit(want)).all())
+    graph = torch.cuda.CUDAGraph()
+    fixed = torch.zeros_like(x)
+    with torch.cuda.graph(graph):
+        held = F.encode_8bit(fixed)
+        values = F.decode_8bit(held)
+    for seed in (6, 7):
+        fixed.copy_(make(x.shape, x.dtype, seed))
+        graph.replay()
+        assert bool((held.codes == F.encode_8bit(fixed).codes).all()) and bool((values == F.decode_8bit(F.encode_8bit(fixed))).all())
+
+
+def test_refusals():
+    x = make((2, 3, 4, 5), torch.float32).cuda()
+    packed = F.encode_8bit(x)
+    for bad in (lambda: F.encode_8bit(x, 0), lambda: F.encode_8bit(x, -1), lambda: F.encode_8bit(x.int()), lambda: F.encode_8bit(x[0, 0, 0, 0]),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales, torch.float64)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes.int(), packed.scales, x.dtype)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales.half(), x.dtype)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales[:1], x.dtype)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales[..., None], x.dtype)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales.cpu(), x.dtype)),
+                lambda: F.decode_8bit(F.Activation8(packed.codes, packed.scales[0, 0, 0], x.dtype))):
+        with pytest.raises(RuntimeError):
+            bad()
+    assert F.encode_8bit(x[0, 0, 0]).scales.shape == (1,)   # fewer dimensions than a row would have
+
+
+# ---- layers that keep their input in 8 bits -------------------------------------------------------------------------------
+
+LAYERS = [(op, merge) for op in ("dilation", "erosion", "smorph") for merge in ("sum", "mean", "max", "min", "identity")] + [("smorph_scm", "sum")]
+
+
+def layer_tensors(op, merge, dtype, shape=(2, 3, 13, 18), Co=4, k=3, seed=0):
+    C = shape[1]
+    Co, Ci = (C, 1) if merge == "identity" else (Co, C)
+    x, w = make(shape, dtype, seed), (make((Co, Ci, k, k), torch.float64, seed + 1) * 0.1).to(dtype)
+    more = []
+    if op.startswith("smorph"):
+        more.append((1 + 0.1 * make((Co, Ci), torch.float64, seed + 2)).to(dtype))
+    if op == "smorph_scm":
+        more.append((0.5 + 0.1 * make((Co,), torch.float64, seed + 3)).to(dtype))
+    return x, w, *more, make((shape[0], Co, *shape[2:]), dtype, seed + 4)
+
+
+def call(op, merge, x, w, *more, save_indices=False):
+    if op == "smorph":
+        return F.smorph, (x, w, *more), dict(channel_merge_mode=merge)
+    if op == "smorph_scm":
+        return F.smorph, (x, w, *more), {}
+    return getattr(F, op), (x, w, merge), dict(save_indices=save_indices)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("op,merge", LAYERS)
+def test_layer_gradients_are_those_at_the_codes(op, merge, dtype):
+    """Output: bit for bit the plain call's. Gradients: those of the plain layer, in double, at the values that the codes stand
+    for. Dilation and erosion add a handful of gradients a pixel, and some hundred a weight, in float: 1e-4 of the largest is the
+    bound that the layers' own tests use; smorph's likewise. Half precision widens to float and rounds the results once."""
+    *tensors, gz = layer_tensors(op, merge, dtype)
+    leaves = [t.cuda().requires_grad_(True) for t in tensors]
+    function, args, kwargs = call(op, merge, *leaves)
+    with torch.no_grad():
+        plain = function(*args, **kwargs)
+    z = F.checkpoint_8bit(function, *args, **kwargs)
+    assert z.dtype == dtype and bool((z == plain).all())
+    got = torch.autograd.grad(z, leaves, gz.cuda())
+
+    # The layer computes in float for half precision, and so does it decode.
+    kept = F.encode_8bit(leaves[0].detach())
+    work = torch.float64 if dtype == torch.float64 else torch.float32
+    values = P.decode(kept.codes.cpu(), kept.scales.cpu(), work)
+    if op in ("dilation", "erosion"):
+        # The winners are those among values as the kernels' type holds them: the oracle in that type, sums of gradients in it.
+        wk = tensors[1].to(work).numpy()
+        wk = wk if op == "dilation" else np.ascontiguousarray(wk[..., ::-1, ::-1])
+        gx, gw = O.morpho_backward(op, values.numpy(), wk, gz.to(work).numpy(), merge)
+        want = [torch.from_numpy(gx), torch.from_numpy(np.ascontiguousarray(gw[..., ::-1, ::-1]) if op == "erosion" else gw)]
+    else:
+        at = [values.double().cuda().requires_grad_(True)] + [t.double().cuda().requires_grad_(True) for t in tensors[1:]]
+        function, args, kwargs = call(op, merge, *at)
+        want = torch.autograd.grad(function(*args, **kwargs), at, gz.double().cuda())
+    tol = 1e-11 if dtype == torch.float64 else 1e-4
+    step = 0.0 if dtype in (torch.float32, torch.float64) else torch.finfo(dtype).eps / 2
+    for a, b in zip(got, want):
+        b = b.cpu().double()
+        assert a.dtype == dtype and a.shape == b.shape
+        bound = tol * max(1.0, float(b.abs().max())) + step * b.abs()
+        assert bool(((a.cpu().double() - b).abs() <= bound).all()), float((a.cpu().double() - b).abs().max())
+
+
+@pytest.mark.parametrize("op", ["dilation", "erosion"])
+@pytest.mark.parametrize("merge", ["max", "min"])
+def test_saved_winners_keep_exact_gradients(op, merge):
+    *tensors, gz = layer_tensors(op, merge, torch.float64)
+    leaves = [t.cuda().requires_grad_(True) for t in tensors]
+    function, args, kwargs = call(op, merge, *leaves, save_indices=True)
+    want = torch.autograd.grad(function(*args, **kwargs), leaves, gz.cuda())
+    z = F.checkpoint_8bit(function, *args, **kwargs)
+    kept = [t for t in z.grad_fn.saved_tensors] if hasattr(z.grad_fn, "saved_tensors") else []
+    assert all(t is None or t.dtype != torch.int8 for t in kept)
+    for a, b in zip(torch.autograd.grad(z, leaves, gz.cuda()), want):
+        assert bool(((a - b).abs() <= 1e-12 * (1 + b.abs())).all())   # atomic sums of a few terms, in double
+
+
+@pytest.mark.parametrize("op,merge", [("dilation", "sum"), ("erosion", "identity"), ("dilation", "max"), ("smorph", "mean"), ("smorph", "identity"),
+                                      ("smorph_scm", "sum"), ("sigma_layer", "sum")])
+def test_gradients_against_differences(op, merge):
+    """At an input that its codes give back, the gradients are those of the layer itself, so that differences show them."""
+    *tensors, gz = layer_tensors("smorph" if op == "sigma_layer" else op, merge, torch.float64, (1, 2, 5, 6), 3)
+    x = tensors[0].cuda()
+    for _ in range(2):
+        x = F.decode_8bit(F.encode_8bit(x))
+    # Distinct sums x + w: a tie has no gradient to compare with.
+    leaves = [x.requires_grad_(True)] + [t.cuda().requires_grad_(True) for t in tensors[1:]]
+
+    def layer(*t):
+        if op == "sigma_layer":
+            return F.checkpoint_8bit(F.sigma_layer, *t, merge, padding_mode="geodesic", save_indices=False)
+        function, args, kwargs = call(op, merge, *t)
+        if op in ("dilation", "erosion"):   # a border pixel that wins by way of the padding gets no gradient: none here
+            kwargs["padding_mode"] = "geodesic"
+        return F.checkpoint_8bit(function, *args, **kwargs)
+
+    assert torch.autograd.gradcheck(layer, leaves, eps=1e-6, atol=1e-5, nondet_tol=1e-10)
+
+
+@pytest.mark.parametrize("shape,k", [((1, 1, 1, 1), 3), ((3, 2, 1, 1), 3), ((2, 3, 1, 7), 5), ((1, 2, 40, 33), 11), ((5, 6, 7, 7), 3), ((2, 2, 9, 9), 2)])
+def test_layer_sizes(shape, k):
+    """Planes of one pixel (one scale an image), of odd sizes, smaller than the structuring element."""
+    for op, merge in (("dilation", "sum"), ("smorph", "mean"), ("erosion", "identity")):
+        *tensors, gz = layer_tensors(op, merge, torch.float64, shape, 3, k)
+        leaves = [t.cuda().requires_grad_(True) for t in tensors]
+        kept = F.decode_8bit(F.encode_8bit(leaves[0].detach(), 3 if shape[2:] == (1, 1) else 2))
+        function, args, kwargs = call(op, merge, *leaves)
+        got = torch.autograd.grad(F.checkpoint_8bit(function, *args, **kwargs), leaves, gz.cuda())
+        at = [kept.requires_grad_(True)] + leaves[1:]
+        function, args, kwargs = call(op, merge, *at)
+        for a, b in zip(got, torch.autograd.grad(function(*args, **kwargs), at, gz.cuda())):
+            assert bool(((a - b).abs() <= 1e-11 * max(1.0, float(b.abs().max()))).all())
+
+
+def test_fewer_dimensions_and_empty_batches():
+    w = make((3, 2, 3, 3), torch.float32, 1).cuda().requires_grad_(True)
+    x = make((2, 6, 7), torch.float32).cuda().requires_grad_(True)
+    gx, gw = torch.autograd.grad(F.checkpoint_8bit(F.dilation, x, w).sum(), (x, w))
+    assert gx.shape == x.shape and gw.shape == w.shape
+    kept = F.decode_8bit(F.encode_8bit(x.detach())).requires_grad_(True)
+    assert bool((gx - torch.autograd.grad(F.dilation(kept, w).sum(), kept)[0]).abs().max() <= 1e-5)
+    plane, square = make((6, 7), torch.float32).cuda().requires_grad_(True), make((3, 3), torch.float32).cuda().requires_grad_(True)
+    gx, gw = torch.autograd.grad(F.checkpoint_8bit(F.erosion, plane, square, "identity").sum(), (plane, square))
+    assert gx.shape == (6, 7) and gw.shape == (3, 3)
+    empty = torch.zeros(0, 2, 6, 7, device="cuda", requires_grad=True)
+    gx, gw = torch.autograd.grad(F.checkpoint_8bit(F.dilation, empty, w).sum(), (empty, w))
+    assert gx.shape == empty.shape and bool((gw == 0).all())
+
+
+@pytest.mark.parametrize("padding", ["zero", "geodesic", "constant", "replicate"])
+def test_masked_inputs_and_padding(padding):
+    """-inf in the input (what a geodesic border or a dropped weight leaves behind) stays out of the winners and out of its
+    block's scale."""
+    x = make((2, 3, 10, 17), torch.float32, 8)
+    x[torch.rand(x.shape, generator=torch.Generator().manual_seed(9)) < 0.2] = -float("inf")
+    w, gz = make((4, 3, 3, 3), torch.float32, 10) * 0.1, make((2, 4, 10, 17), torch.float32, 11)
+    leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)]
+    z = F.checkpoint_8bit(F.dilation, *leaves, "sum", padding, padding_value=0.25)
+    got = torch.autograd.grad(z, leaves, gz.cuda())
+    kept = F.encode_8bit(x.cuda())
+    values = P.decode(kept.codes.cpu(), kept.scales.cpu(), torch.float32)
+    assert bool((values.isinf() == x.isinf()).all())
+    gx, gw = O.morpho_backward("dilation", values.numpy(), w.numpy(), gz.numpy(), "sum", padding, 0.25)
+    np.testing.assert_allclose(got[0].cpu().numpy(), gx, rtol=1e-4, atol=1e-4)
+    np.testing.assert_allclose(got[1].cpu().numpy(), gw, rtol=1e-4, atol=1e-3)
+
+
+def test_what_is_kept():
+    """The graph holds codes and no float tensor of the input's size, the input may change before the backward pass, no_grad
+    encodes nothing, and a module or a model is called like a function."""
+    x = make((4, 8, 64, 64), torch.float32).cuda().requires_grad_(True)
+    layer = Mnn.Dilation(8, 8, 3, "identity").cuda()
+    torch.nn.init.normal_(layer.weight, std=0.1)
+
+    def allocated_by(f):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        kept = f()
+        return torch.cuda.memory_allocated() - before, kept
+
+    hidden = (x * 1.0)
+    size = hidden.nbytes
+    plain, a = allocated_by(lambda: layer(x * 1.0))
+    packed, b = allocated_by(lambda: F.checkpoint_8bit(layer, x * 1.0))
+    assert plain >= 2 * size and packed <= size + size * 0.27
+    g = torch.randn_like(a)
+    want = torch.autograd.grad(layer(F.decode_8bit(F.encode_8bit(x.detach())).requires_grad_(True)), layer.weight, g)[0]
+    hidden = x.detach().clone()
+    z = F.checkpoint_8bit(layer, hidden)
+    hidden.zero_()
+    assert bool((torch.autograd.grad(z, layer.weight, g)[0] - want).abs().max() <= 1e-3)
+    from morphocore_b200 import _native
+    with torch.no_grad():
+        layer(x)
+        before = _native.launch_count()
+        layer(x)
+        one = _native.launch_count() - before
+        F.checkpoint_8bit(layer, x)
+        assert _native.launch_count() - before == 2 * one
+    model = torch.nn.Sequential(Mnn.Opening(8, 8, 3), Mnn.SigmaLayer(8, 8, 3), Mnn.RMSNorm(8), Mnn.SMorph(8, 4, 3, init_alpha=1.0)).cuda()
+    out = F.checkpoint_8bit(model, x)
+    assert bool((out == model(x)).all())
+    out.square().mean().backward()
+    assert all(p.grad is not None and bool(p.grad.isfinite().all()) for p in model.parameters())
+
+
+def test_packed_input_of_a_layer():
+    x = make((2, 4, 9, 14), torch.float32, 3).cuda().requires_grad_(True)
+    w = (make((4, 4, 3, 3), torch.float32, 4) * 0.1).cuda().requires_grad_(True)
+    alpha = torch.full((4, 4), 1.5, device="cuda")
+    other = F.encode_8bit(x.detach() * 2)   # not that of x: what is used shows
+    g = torch.randn(2, 4, 9, 14, device="cuda")
+    at = F.decode_8bit(other).requires_grad_(True)
+    for function, more in ((F.dilation, ("sum",)), (F.smorph, (alpha,)), (F.sigma_layer, (alpha, "max")), (F.sigma_layer, (alpha, "sum", "replicate", False))):
+        with torch.no_grad():
+            plain = function(x, w, *more)
+        z = F.checkpoint_8bit(function, x, w, *more, packed=other)
+        assert bool((z == plain).all())
+        got = torch.autograd.grad(z, (x, w), g)
+        want = torch.autograd.grad(function(at if more[-1] != "max" else x, w, *more), (at if more[-1] != "max" else x, w), g)
+        for a, b in zip(got, want):
+            assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+    # Codes of a token's layout decode by their own rows.
+    rows = F.encode_8bit(x.detach(), 3)
+    assert rows.scales.shape == (2, 4)
+    torch.autograd.grad(F.checkpoint_8bit(F.dilation, x, w, packed=rows), (x, w), g)
+    half = F.encode_8bit(x.detach().half())
+    for bad in (F.encode_8bit(x.detach()[:1]), F.encode_8bit(x.detach().double()), F.Activation8(other.codes, other.scales[:, :2], x.dtype),
+                F.Activation8(other.codes.cpu(), other.scales, x.dtype)):
+        with pytest.raises(RuntimeError):
+            F.checkpoint_8bit(F.dilation, x, w, packed=bad)
+    xh, wh = x.detach().half().requires_grad_(True), w.detach().half().requires_grad_(True)
+    assert torch.autograd.grad(F.checkpoint_8bit(F.dilation, xh, wh, packed=half), xh, g.half())[0].dtype == torch.float16
+
+
+def test_noise_and_dropout_in_8_bits():
+    """What is drawn in the call is drawn as in the plain call, and the gradients are those of that draw at the codes."""
+    x = make((3, 4, 9, 11), torch.float32, 3).cuda().requires_grad_(True)
+    w = (make((4, 4, 3, 3), torch.float32, 4) * 0.1).cuda().requires_grad_(True)
+    g = make((3, 4, 9, 11), torch.float32, 5).cuda()
+    for function in (F.dilation, F.erosion):
+        for kwargs in (dict(noise_scale=0.2), dict(weight_dropout=0.3)):
+            def drawn(call, x):
+                torch.manual_seed(11)
+                return call(x, w, training=True, **kwargs)
+
+            z = drawn(lambda *t, **k: F.checkpoint_8bit(function, *t, **k), x)
+            assert bool((z == drawn(function, x)).all())
+            kept = F.decode_8bit(F.encode_8bit(x.detach())).requires_grad_(True)
+            # The same kernels on the same numbers, atomic sums in float.
+            for a, b in zip(torch.autograd.grad(z, (x, w), g), torch.autograd.grad(drawn(function, kept), (kept, w), g)):
+                assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+def test_training_step_in_a_graph():
+    """Forward and backward under checkpoint_8bit, captured and replayed on new data."""
+    w = (make((4, 4, 3, 3), torch.float32, 4) * 0.1).cuda().requires_grad_(True)
+    alpha = torch.full((4, 4), 1.5, device="cuda", requires_grad=True)
+    fixed, g = torch.zeros(2, 4, 16, 20, device="cuda", requires_grad=True), torch.randn(2, 4, 16, 20, device="cuda")
+
+    def step(x, w, alpha):
+        return torch.autograd.grad(F.checkpoint_8bit(F.smorph, x, w, alpha), (x, w, alpha), g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(fixed, w, alpha)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step(fixed, w, alpha)
+    for seed in (1, 2):
+        x = make(fixed.shape, torch.float32, seed).cuda()
+        with torch.no_grad():
+            fixed.copy_(x)
+        graph.replay()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, step(x.requires_grad_(True), w.detach().requires_grad_(True), alpha.detach().requires_grad_(True))):
+            assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
