@@ -13,6 +13,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace mc
@@ -25,81 +27,159 @@ template <typename T> struct WideOf { using type = float; };
 template <> struct WideOf<double> { using type = double; };
 template <typename T> using Wide = typename WideOf<T>::type;
 
+/// One element of a parameter.
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ double widen(double v) { return v; }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-/// Rounded to T, to nearest even.
 template <typename T> __device__ __forceinline__ T narrow(Wide<T> v);
 template <> __device__ __forceinline__ float narrow<float>(float v) { return v; }
 template <> __device__ __forceinline__ double narrow<double>(double v) { return v; }
 template <> __device__ __forceinline__ __half narrow<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 narrow<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-/// Four elements of a lane, as they lie in memory. The widest loads are of 16 bytes.
-template <typename T> struct alignas(sizeof(T) == 8 ? 16 : 4 * sizeof(T)) Quad
+/// Four elements of a lane, as they lie in memory; the widest loads are of 16 bytes. Half precision stays packed until it is widened: taking
+/// the halves apart where they are loaded would make every conditional load wait for its data (encoding bfloat16 took 132 us where
+/// float takes 84 on the same number of elements).
+template <typename T> struct alignas(16) Quad
 {
     T e[4];
 };
-
-/// Position within the block of a lane's element k.
-template <bool VEC> __device__ __forceinline__ int quad_at(int lane, int k) { return VEC ? 4 * lane + k : lane + 32 * k; }
-
-/// A lane's elements of the block at `src`, of which `valid` exist (a multiple of four if VEC); zeros past them.
-template <bool VEC, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* src, int lane, int valid)
+struct alignas(8) PackedQuad
 {
-    Quad<T> q;
-    if constexpr (VEC)
+    uint32_t word[2];
+};
+template <> struct alignas(8) Quad<__half> : PackedQuad
+{
+};
+template <> struct alignas(8) Quad<__nv_bfloat16> : PackedQuad
+{
+};
+
+template <typename T> __device__ __forceinline__ void widen_quad(const Quad<T>& q, Wide<T> (&v)[4])
+{
+    if constexpr (std::is_same<T, __half>::value)
     {
-        if (4 * lane < valid) q = *reinterpret_cast<const Quad<T>*>(src + 4 * lane);
-        else
 #pragma unroll
-            for (int k = 0; k < 4; k++) q.e[k] = T(0.0f);
+        for (int h = 0; h < 2; h++)
+        {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&q.word[h]));
+            v[2 * h] = f.x;
+            v[2 * h + 1] = f.y;
+        }
+    }
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+        {
+            v[2 * h] = __uint_as_float(q.word[h] << 16);
+            v[2 * h + 1] = __uint_as_float(q.word[h] & 0xffff0000u);
+        }
     }
     else
 #pragma unroll
-        for (int k = 0; k < 4; k++) q.e[k] = lane + 32 * k < valid ? src[lane + 32 * k] : T(0.0f);
+        for (int k = 0; k < 4; k++) v[k] = q.e[k];
+}
+
+/// Rounded to T, to nearest even.
+template <typename T> __device__ __forceinline__ Quad<T> narrow_quad(const Wide<T> (&v)[4])
+{
+    Quad<T> q;
+    if constexpr (std::is_same<T, __half>::value)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+        {
+            const __half2 pair = __floats2half2_rn(v[2 * h], v[2 * h + 1]);
+            q.word[h] = *reinterpret_cast<const uint32_t*>(&pair);
+        }
+    }
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value)
+    {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+        {
+            const __nv_bfloat162 pair = __floats2bfloat162_rn(v[2 * h], v[2 * h + 1]);
+            q.word[h] = *reinterpret_cast<const uint32_t*>(&pair);
+        }
+    }
+    else
+#pragma unroll
+        for (int k = 0; k < 4; k++) q.e[k] = v[k];
     return q;
 }
 
-template <bool VEC, typename T> __device__ __forceinline__ void store_quad(T* dst, const Quad<T>& q, int lane, int valid)
+/// Position within the block of a lane's first element; and of element k.
+template <bool VEC> __device__ __forceinline__ int lane_at(int lane) { return VEC ? 4 * lane : lane; }
+template <bool VEC> __device__ __forceinline__ int quad_at(int lane, int k) { return lane_at<VEC>(lane) + (VEC ? k : 32 * k); }
+
+// The four functions below take the address of the lane's first element and how many elements of the block lie from there on: with
+// VEC all four of a lane exist (left > 0) or none, otherwise element k does where 32 k < left.
+
+/// A lane's elements; zeros where there are none.
+template <bool VEC, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* src, int left)
+{
+    Quad<T> q{};
+    if constexpr (VEC)
+    {
+        if (left > 0) q = *reinterpret_cast<const Quad<T>*>(src);
+    }
+    else if constexpr (sizeof(T) == 2)
+    {
+        uint32_t half[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) half[k] = 32 * k < left ? reinterpret_cast<const uint16_t*>(src)[32 * k] : 0u;
+#pragma unroll
+        for (int h = 0; h < 2; h++) q.word[h] = half[2 * h] | half[2 * h + 1] << 16;
+    }
+    else
+#pragma unroll
+        for (int k = 0; k < 4; k++) q.e[k] = 32 * k < left ? src[32 * k] : T(0);
+    return q;
+}
+
+template <bool VEC, typename T> __device__ __forceinline__ void store_quad(T* dst, const Quad<T>& q, int left)
 {
     if constexpr (VEC)
     {
-        if (4 * lane < valid) *reinterpret_cast<Quad<T>*>(dst + 4 * lane) = q;
+        if (left > 0) *reinterpret_cast<Quad<T>*>(dst) = q;
     }
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (lane + 32 * k < valid) dst[lane + 32 * k] = q.e[k];
+            if (32 * k < left)
+            {
+                if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(dst)[32 * k] = static_cast<uint16_t>(q.word[k / 2] >> (16 * (k % 2)));
+                else dst[32 * k] = q.e[k];
+            }
 }
 
 /// A lane's four codes, element k in byte k.
-template <bool VEC> __device__ __forceinline__ uint32_t load_codes(const int8_t* src, int lane, int valid)
+template <bool VEC> __device__ __forceinline__ uint32_t load_codes(const int8_t* src, int left)
 {
     uint32_t q = 0;
     if constexpr (VEC)
     {
-        if (4 * lane < valid) q = *reinterpret_cast<const uint32_t*>(src + 4 * lane);
+        if (left > 0) q = *reinterpret_cast<const uint32_t*>(src);
     }
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (lane + 32 * k < valid) q |= static_cast<uint32_t>(static_cast<uint8_t>(src[lane + 32 * k])) << (8 * k);
+            if (32 * k < left) q |= static_cast<uint32_t>(static_cast<uint8_t>(src[32 * k])) << (8 * k);
     return q;
 }
 
-template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* dst, uint32_t codes, int lane, int valid)
+template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* dst, uint32_t codes, int left)
 {
     if constexpr (VEC)
     {
-        if (4 * lane < valid) *reinterpret_cast<uint32_t*>(dst + 4 * lane) = codes;
+        if (left > 0) *reinterpret_cast<uint32_t*>(dst) = codes;
     }
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (lane + 32 * k < valid) dst[lane + 32 * k] = static_cast<int8_t>(codes >> (8 * k));
+            if (32 * k < left) dst[32 * k] = static_cast<int8_t>(codes >> (8 * k));
 }
 
 __device__ __forceinline__ uint32_t pack_bytes(const uint32_t (&q)[4])
@@ -107,54 +187,103 @@ __device__ __forceinline__ uint32_t pack_bytes(const uint32_t (&q)[4])
     return __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
 }
 
+/// First statement of a branch that is hardly ever taken: keeps the compiler from computing both sides and selecting, which would cost
+/// every element the instructions of the exception (encoding bfloat16 issued 19 instructions an element instead of 7).
+__device__ __forceinline__ void rarely() { asm volatile(""); }
+
 /// Code of a value without a number: -128 for NaN, -127 and 127 for the infinities.
 template <typename W> __device__ __forceinline__ uint32_t code_of_nonfinite(W v) { return v != v ? 0x80u : (v > W(0) ? 0x7fu : 0x81u); }
 
-/// Codes of the block that the warp holds (absent elements are zeros), and its scale, the same in every lane. Called by whole
-/// warps. The rounding is that of one fused multiply-add: x * (126 / m) + 1.5 * 2^23 has the whole number in its low bits.
-__device__ __forceinline__ uint32_t encode_quad(const float (&v)[4], float& scale)
+/// Scale and 126 / m of a block whose largest finite magnitude is m.
+__device__ __forceinline__ void block_scale(float m, float& scale, float& inverse)
 {
-    constexpr uint32_t INF = 0x7f800000u;
-    uint32_t bits[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) bits[k] = __float_as_uint(v[k]) & 0x7fffffffu;
-    uint32_t top = __reduce_max_sync(0xffffffffu, max(max(bits[0], bits[1]), max(bits[2], bits[3])));
-    const bool all_finite = top < INF;
-    if (!all_finite)
-    {
-        top = 0;
-#pragma unroll
-        for (int k = 0; k < 4; k++) top = bits[k] < INF ? max(top, bits[k]) : top;
-        top = __reduce_max_sync(0xffffffffu, top);
-    }
-    const float m = __uint_as_float(top);
     const bool none = m < 0x1p-100f;
-    const float inverse = none ? 0.0f : __fdiv_rn(126.0f, m);
+    inverse = none ? 0.0f : __fdiv_rn(126.0f, m);
     scale = none ? 0.0f : m * (1.0f / 126.0f);
-    uint32_t q[4];
-#pragma unroll
-    for (int k = 0; k < 4; k++) q[k] = __float_as_uint(fmaf(v[k], inverse, 12582912.0f));
-    if (!all_finite)
-#pragma unroll
-        for (int k = 0; k < 4; k++) q[k] = bits[k] < INF ? q[k] : code_of_nonfinite(v[k]);
-    return pack_bytes(q);
 }
 
-__device__ __forceinline__ uint32_t encode_quad(const double (&v)[4], double& scale)
+/// Codes of N blocks that the warp holds, four elements of each a lane (absent elements are zeros). Lane i < N returns the scale of
+/// block i. Called by whole warps. The rounding is that of one fused multiply-add: x * (126 / m) + 1.5 * 2^23 has the whole number in
+/// its low bits. The division, a dozen instructions that a warp would repeat for every block, is done once: lane i does that of
+/// block i.
+template <int N> __device__ __forceinline__ float encode_blocks(const float (&v)[N][4], uint32_t (&codes)[N], int lane)
 {
-    double m = 0.0;
+    constexpr uint32_t INF = 0x7f800000u;
+    uint32_t top[N], largest = 0, mine = 0;
 #pragma unroll
-    for (int k = 0; k < 4; k++) m = isfinite(v[k]) ? fmax(m, fabs(v[k])) : m;
+    for (int i = 0; i < N; i++)
+    {
+        uint32_t m = 0;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, d));
-    const bool none = m < 0x1p-900;
-    const double inverse = none ? 0.0 : 126.0 / m;
-    scale = none ? 0.0 : m * (1.0 / 126.0);
-    uint32_t q[4];
+        for (int k = 0; k < 4; k++) m = max(m, __float_as_uint(v[i][k]) & 0x7fffffffu);
+        top[i] = __reduce_max_sync(0xffffffffu, m);
+        largest = max(largest, top[i]);
+    }
+    const bool all_finite = largest < INF;
+    if (!all_finite)
+    {
+        rarely();
 #pragma unroll
-    for (int k = 0; k < 4; k++)
-        q[k] = isfinite(v[k]) ? static_cast<uint32_t>(__double2loint(fma(v[k], inverse, 6755399441055744.0))) : code_of_nonfinite(v[k]);
-    return pack_bytes(q);
+        for (int i = 0; i < N; i++)
+        {
+            uint32_t m = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+            {
+                const uint32_t bits = __float_as_uint(v[i][k]) & 0x7fffffffu;
+                m = bits < INF ? max(m, bits) : m;
+            }
+            top[i] = __reduce_max_sync(0xffffffffu, m);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; i++) mine = lane == i ? top[i] : mine;
+    float scale, inverse;
+    block_scale(__uint_as_float(mine), scale, inverse);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+    {
+        const float of_block = __shfl_sync(0xffffffffu, inverse, i);
+        uint32_t q[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) q[k] = __float_as_uint(fmaf(v[i][k], of_block, 12582912.0f));
+        if (!all_finite)
+        {
+            rarely();
+#pragma unroll
+            for (int k = 0; k < 4; k++) q[k] = (__float_as_uint(v[i][k]) & 0x7fffffffu) < INF ? q[k] : code_of_nonfinite(v[i][k]);
+        }
+        codes[i] = pack_bytes(q);
+    }
+    return scale;
+}
+
+template <int N> __device__ __forceinline__ double encode_blocks(const double (&v)[N][4], uint32_t (&codes)[N], int lane)
+{
+    double mine = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; i++)
+    {
+        double m = 0.0;
+#pragma unroll
+        for (int k = 0; k < 4; k++) m = isfinite(v[i][k]) ? fmax(m, fabs(v[i][k])) : m;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) m = fmax(m, __shfl_xor_sync(0xffffffffu, m, d));
+        mine = lane == i ? m : mine;
+    }
+    const bool none = mine < 0x1p-900;
+    const double inverse = none ? 0.0 : 126.0 / mine, scale = none ? 0.0 : mine * (1.0 / 126.0);
+#pragma unroll
+    for (int i = 0; i < N; i++)
+    {
+        const double of_block = __shfl_sync(0xffffffffu, inverse, i);
+        uint32_t q[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            q[k] = isfinite(v[i][k]) ? static_cast<uint32_t>(__double2loint(fma(v[i][k], of_block, 6755399441055744.0))) : code_of_nonfinite(v[i][k]);
+        codes[i] = pack_bytes(q);
+    }
+    return scale;
 }
 
 /// Code k of four as a number: its byte becomes the low mantissa byte of 2^23 + 128 + code.
@@ -163,18 +292,32 @@ __device__ __forceinline__ float code_value(uint32_t codes, int k)
     return __uint_as_float(__byte_perm(codes ^ 0x80808080u, 0x4B000000u, 0x7540u | static_cast<uint32_t>(k))) - 8388736.0f;
 }
 
-/// What code k of a block with this scale stands for.
-__device__ __forceinline__ float decode_code(uint32_t codes, int k, float scale)
+/// What a lane's four codes of a block with this scale stand for.
+__device__ __forceinline__ void decode_quad(uint32_t codes, float scale, float (&v)[4])
 {
-    const float q = code_value(codes, k);
-    if (fabsf(q) > 126.0f) return q < -127.0f ? __uint_as_float(0x7fc00000u) : copysignf(__uint_as_float(0x7f800000u), q);
-    return q * scale;
+    float q[4];
+#pragma unroll
+    for (int k = 0; k < 4; k++) q[k] = code_value(codes, k);
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = q[k] * scale;
+    if (fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3]))) > 126.0f)
+    {
+        rarely();
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (fabsf(q[k]) > 126.0f) v[k] = q[k] < -127.0f ? __uint_as_float(0x7fc00000u) : copysignf(__uint_as_float(0x7f800000u), q[k]);
+    }
 }
-__device__ __forceinline__ double decode_code(uint32_t codes, int k, double scale)
+__device__ __forceinline__ void decode_quad(uint32_t codes, double scale, double (&v)[4])
 {
-    const double q = code_value(codes, k);
-    if (fabs(q) > 126.0) return q < -127.0 ? __longlong_as_double(0x7ff8000000000000ll) : copysign(__longlong_as_double(0x7ff0000000000000ll), q);
-    return q * scale;
+#pragma unroll
+    for (int k = 0; k < 4; k++)
+    {
+        const float q = code_value(codes, k);
+        v[k] = static_cast<double>(q) * scale;
+        if (fabsf(q) > 126.0f)
+            v[k] = q < -127.0f ? __longlong_as_double(0x7ff8000000000000ll) : copysign(__longlong_as_double(0x7ff0000000000000ll), static_cast<double>(q));
+    }
 }
 
 /// Calls f(T{}) for the type an mc_dtype names.

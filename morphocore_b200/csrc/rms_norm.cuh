@@ -8,11 +8,13 @@
 // rows of channels (rows), stays in registers between the sums over the channels and what is computed from them. Bytes bound
 // them: a forward pass with residual moves 16 bytes an element in float (13 with the result in 8 bits), a backward pass 16 (13).
 //
-// The sums over the channels are taken in double and y is rounded once, from an unevaluated sum of two floats that carries about
-// 46 bits: y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and in
-// whatever order (a float that is one unit off moves one code in 10^5 to its neighbour). A conversion to double and a fused
-// multiply-add an element are a third of what their units do while the bytes of the element pass.
+// In float the sums over the channels are taken in double and y is rounded once, from an unevaluated sum of two floats that carries
+// about 46 bits: y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
+// in whatever order (a float that is one unit off moves one code in 10^5 to its neighbour). In half precision both are plain float:
+// what is left of its three half steps after the rounding to 8 or 11 bits is one result in 2^13 or 2^10 that goes to the other neighbour.
 #pragma once
+#include <type_traits>
+
 #include "encode8.cuh"
 
 namespace mc
@@ -39,19 +41,68 @@ struct NormGradArgs
     double eps;
 };
 
-/// s r g in the type that T is computed in, rounded once (see above). `fast`: every r of the warp lies within 2^-60 .. 2^60, so that
-/// its two halves are ordinary floats and an infinite s cannot meet them (its r is 0).
-__device__ __forceinline__ float scaled_value(float s, double r, float g, bool fast)
+/// What the forward kernels add squares up in.
+template <typename T> struct SumOf { using type = double; };
+template <> struct SumOf<__half> { using type = float; };
+template <> struct SumOf<__nv_bfloat16> { using type = float; };
+template <typename T> using Sum = typename SumOf<T>::type;
+
+/// The factor r of a lane's elements as the products with it are taken, for an ordinary r: the halves are normal floats, and an
+/// infinite s cannot meet them (its r is 0). `times` rounds s r g once to float for float (r as two floats with about 48 bits of it,
+/// pairs of elements by packed instructions) and after each product otherwise.
+template <typename T> struct Factor
 {
-    if (!fast) return static_cast<float>(static_cast<double>(s) * r * static_cast<double>(g));
-    const float high = static_cast<float>(r), low = static_cast<float>(r - static_cast<double>(high));
-    const float p = s * high, p_low = fmaf(s, low, fmaf(s, high, -p));
-    const float y = p * g;
-    return fabsf(y) <= Limits<float>::max() ? y + fmaf(p_low, g, fmaf(p, g, -y)) : y;   // an infinite product has no remainder
+    Wide<T> r;
+    __device__ __forceinline__ void set(double v) { r = static_cast<Wide<T>>(v); }
+};
+template <> struct Factor<float>
+{
+    float r, low;
+    __device__ __forceinline__ void set(double v)
+    {
+        r = static_cast<float>(v);
+        low = static_cast<float>(v - static_cast<double>(r));
+    }
+};
+
+template <typename T> __device__ __forceinline__ void times(const Wide<T> (&s)[4], const Factor<T>& r0, const Factor<T>& r1, const Factor<T>& r2,
+                                                            const Factor<T>& r3, const Wide<T> (&g)[4], Wide<T> (&y)[4])
+{
+    if constexpr (std::is_same<T, float>::value)
+    {
+        const auto pair = [](float s0, float s1, const Factor<float>& a, const Factor<float>& b, float g0, float g1, float& y0, float& y1) {
+            const float2 v = make_float2(s0, s1), g = make_float2(g0, g1);
+            const float2 p = __fmul2_rn(v, make_float2(a.r, b.r));
+            const float2 p_low = __ffma2_rn(v, make_float2(a.low, b.low), __ffma2_rn(v, make_float2(a.r, b.r), make_float2(-p.x, -p.y)));
+            const float2 y = __fmul2_rn(p, g);
+            const float2 sum = __fadd2_rn(y, __ffma2_rn(p_low, g, __ffma2_rn(p, g, make_float2(-y.x, -y.y))));
+            y0 = sum.x;
+            y1 = sum.y;
+        };
+        pair(s[0], s[1], r0, r1, g[0], g[1], y[0], y[1]);
+        pair(s[2], s[3], r2, r3, g[2], g[3], y[2], y[3]);
+    }
+    else
+    {
+        y[0] = s[0] * r0.r * g[0];
+        y[1] = s[1] * r1.r * g[1];
+        y[2] = s[2] * r2.r * g[2];
+        y[3] = s[3] * r3.r * g[3];
+    }
 }
-__device__ __forceinline__ double scaled_value(double s, double r, double g, bool) { return s * r * g; }
+
+/// Whether the products above hold with weights of this size: an infinite product has no remainder.
+__device__ __forceinline__ bool ordinary_weight(float g) { return fabsf(g) < 0x1p100f; }
+__device__ __forceinline__ bool ordinary_weight(double) { return true; }
 
 __device__ __forceinline__ bool ordinary(double r) { return r > 0x1p-60 && r < 0x1p60; }
+
+/// Sums in float are taken once more in double where they left its range: squares near its largest value, or, for an eps that does not
+/// cover them, near its smallest; infinities and NaN.
+__device__ __forceinline__ bool out_of_range(double squares, double products, double eps)
+{
+    return !(squares < 0x1p120) || (squares < 0x1p-60 && eps < 0x1p-60) || !(fabs(products) < 0x1p120);
+}
 
 __device__ __forceinline__ double warp_sum(double v)
 {
@@ -69,130 +120,182 @@ __device__ __forceinline__ float warp_sum(float v)
 /// x + residual, rounded to T.
 template <typename T> __device__ __forceinline__ Quad<T> add_quads(const Quad<T>& a, const Quad<T>& b)
 {
-    Quad<T> s;
+    Wide<T> u[4], v[4];
+    widen_quad(a, u);
+    widen_quad(b, v);
 #pragma unroll
-    for (int k = 0; k < 4; k++) s.e[k] = narrow<T>(widen(a.e[k]) + widen(b.e[k]));
-    return s;
+    for (int k = 0; k < 4; k++) u[k] += v[k];
+    return narrow_quad<T>(u);
 }
 
-template <typename T> __device__ __forceinline__ void widen_quad(const Quad<T>& q, Wide<T> (&v)[4])
+/// Sums of squares of N quads, one a lane's element or one for all four, added to `sums`.
+template <int N, int SUMS, typename T, typename S> __device__ __forceinline__ void add_squares(const Quad<T> (&s)[N], S (&sums)[SUMS])
 {
 #pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = widen(q.e[k]);
-}
-
-/// Writes the codes and the scale of a block held as a quad.
-template <bool VEC, typename T>
-__device__ __forceinline__ void put_codes(int8_t* codes, void* scales, int64_t at, int64_t block, const Quad<T>& q, int lane, int valid)
-{
-    Wide<T> v[4], scale;
-    widen_quad(q, v);
-    const uint32_t c = encode_quad(v, scale);
-    store_codes<VEC>(codes + at, c, lane, valid);
-    if (lane == 0) static_cast<Wide<T>*>(scales)[block] = scale;
-}
-
-/// Writes y, and its codes, of a block of s. `r` holds the factor of each of the lane's elements, `g` their weights.
-template <bool VEC, typename T>
-__device__ __forceinline__ void put_result(const NormArgs& a, const Quad<T>& s, const double (&r)[4], const Wide<T> (&g)[4], bool fast, int64_t at,
-                                           int64_t block, int lane, int valid)
-{
-    Quad<T> y;
+    for (int i = 0; i < N; i++)
+    {
+        Wide<T> v[4];
+        widen_quad(s[i], v);
 #pragma unroll
-    for (int k = 0; k < 4; k++) y.e[k] = narrow<T>(scaled_value(widen(s.e[k]), r[k], g[k], fast));
-    if (a.y != nullptr) store_quad<VEC>(static_cast<T*>(a.y) + at, y, lane, valid);
-    if (a.y_codes != nullptr) put_codes<VEC>(a.y_codes, a.y_scales, at, block, y, lane, valid);
+        for (int k = 0; k < 4; k++) sums[k % SUMS] = fma(static_cast<S>(v[k]), static_cast<S>(v[k]), sums[k % SUMS]);
+    }
 }
 
-/// s of a block: x, or x + residual, which is stored.
-template <bool VEC, typename T> __device__ __forceinline__ Quad<T> take_sum(const NormArgs& a, int64_t at, int lane, int valid)
+/// Codes and scales of N blocks, of which the first of lane and the others `step` elements and `block_step` blocks apart; `count` exist.
+/// `scales` is where the scale of the first goes.
+template <bool VEC, int N, typename T>
+__device__ __forceinline__ void put_codes(int8_t* codes, void* scales, int64_t step, int64_t block_step, const Quad<T> (&q)[N], int count, int lane, const int (&left)[N])
 {
-    const Quad<T> x = load_quad<VEC>(static_cast<const T*>(a.x) + at, lane, valid);
-    if (a.residual == nullptr) return x;
-    return add_quads(x, load_quad<VEC>(static_cast<const T*>(a.residual) + at, lane, valid));
+    Wide<T> v[N][4];
+    uint32_t c[N];
+#pragma unroll
+    for (int i = 0; i < N; i++) widen_quad(q[i], v[i]);
+    const Wide<T> scale = encode_blocks(v, c, lane);
+#pragma unroll
+    for (int i = 0; i < N; i++) store_codes<VEC>(codes + i * step, c[i], left[i]);
+    if (lane < count) static_cast<Wide<T>*>(scales)[lane * block_step] = scale;
 }
 
-/// Elements of block j of a row of C (negative or zero past its end; the loads take that as none).
-__device__ __forceinline__ int present(int j, int C) { return min(CODE_BLOCK, C - j * CODE_BLOCK); }
+/// Blocks are finished and encoded this many at a time.
+constexpr int GROUP = 4;
 
 /// Forward, feature maps. A block of WARPS warps takes 128 pixels of an image; warp w has the channels w, w + WARPS, ... and keeps
 /// up to HELD of them. Where there are more, the second pass reads s again, from `sum` or x: the tiles that are at work then
 /// lie in L2 (128 pixels of 512 channels in float are 256 KiB, of 296 thread blocks 76 MiB).
-template <typename T, bool VEC, int HELD, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) rms_norm_columns_kernel(const NormArgs a)
+template <typename T, bool VEC, int HELD, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
 {
-    static_assert(WARPS >= 4, "a thread for every pixel of the tile");
+    static_assert(WARPS >= 4 && HELD % GROUP == 0, "a thread for every pixel of the tile");
+    using W = Wide<T>;
     __shared__ double part[WARPS][CODE_BLOCK];
     __shared__ double factor[CODE_BLOCK];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t C = a.channels;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, C = static_cast<int>(a.channels);
+    const int own = (C - warp + WARPS - 1) / WARPS;   // channels of this warp
     const bool held = C <= HELD * WARPS;
+    const int64_t step = WARPS * a.inner, block_step = WARPS * a.tiles_per_row;
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
         const int64_t image = tile / a.tiles_per_row, piece = tile - image * a.tiles_per_row;
-        const int valid = static_cast<int>(min(static_cast<int64_t>(CODE_BLOCK), a.inner - piece * CODE_BLOCK));
-        const int64_t first = image * C * a.inner + piece * CODE_BLOCK, first_block = image * C * a.tiles_per_row + piece;
+        const int left = static_cast<int>(min(static_cast<int64_t>(CODE_BLOCK), a.inner - piece * CODE_BLOCK)) - lane_at<VEC>(lane);
+        const int64_t first = (image * C + warp) * a.inner + piece * CODE_BLOCK + lane_at<VEC>(lane);
+        const int64_t first_block = (image * C + warp) * a.tiles_per_row + piece;
         Quad<T> s[HELD];
-        double sums[4] = {};
-        for (int64_t c0 = warp; c0 < C; c0 += HELD * WARPS)
+        const auto load = [&](const void* from, int i0, Quad<T> (&q)[HELD]) {
+            const T* p = static_cast<const T*>(from) + first + i0 * step;
+#pragma unroll
+            for (int i = 0; i < HELD; i++, p += step) q[i] = load_quad<VEC>(p, i0 + i < own ? left : 0);
+        };
+        Sum<T> sums[4] = {};
+        for (int i0 = 0; i0 < own; i0 += HELD)
         {
-#pragma unroll
-            for (int i = 0; i < HELD; i++)
+            load(a.x, i0, s);
+            if (a.residual != nullptr)
             {
-                const int64_t c = c0 + i * WARPS;
-                s[i] = take_sum<VEC, T>(a, first + c * a.inner, lane, c < C ? valid : 0);
-            }
+                Quad<T> more[HELD];
+                load(a.residual, i0, more);
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
-            {
-                const int64_t c = c0 + i * WARPS;
+                for (int i = 0; i < HELD; i++) s[i] = add_quads(s[i], more[i]);
+                T* p = static_cast<T*>(a.sum) + first + i0 * step;
 #pragma unroll
-                for (int k = 0; k < 4; k++) sums[k] = fma(static_cast<double>(widen(s[i].e[k])), static_cast<double>(widen(s[i].e[k])), sums[k]);
-                if (c >= C) continue;
-                const int64_t at = first + c * a.inner;
-                if (a.residual != nullptr) store_quad<VEC>(static_cast<T*>(a.sum) + at, s[i], lane, valid);
-                if (a.sum_codes != nullptr) put_codes<VEC>(a.sum_codes, a.sum_scales, at, first_block + c * a.tiles_per_row, s[i], lane, valid);
+                for (int i = 0; i < HELD; i++, p += step) store_quad<VEC>(p, s[i], i0 + i < own ? left : 0);
             }
+            add_squares(s, sums);
+            if (a.sum_codes != nullptr)
+#pragma unroll
+                for (int g0 = 0; g0 < HELD; g0 += GROUP)
+                {
+                    const int at = i0 + g0;
+                    if (at >= own) break;
+                    const Quad<T> q[GROUP] = {s[g0], s[g0 + 1], s[g0 + 2], s[g0 + 3]};
+                    const int lefts[GROUP] = {left, at + 1 < own ? left : 0, at + 2 < own ? left : 0, at + 3 < own ? left : 0};
+                    put_codes<VEC>(a.sum_codes + first + at * step, static_cast<W*>(a.sum_scales) + first_block + at * block_step, step, block_step, q,
+                                   own - at, lane, lefts);
+                }
         }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
+        // Squares that left the range of float (half precision only), or would where eps does not cover them: in double.
+        const auto put_sums = [&](auto& from) {
 #pragma unroll
-        for (int k = 0; k < 4; k++) part[warp][quad_at<VEC>(lane, k)] = sums[k];
-        __syncthreads();
-        if (threadIdx.x < CODE_BLOCK)
-        {
+            for (int k = 0; k < 4; k++) part[warp][quad_at<VEC>(lane, k)] = static_cast<double>(from[k]);
+        };
+        put_sums(sums);
+        const auto put_factor = [&]() {
             double total = 0.0;
 #pragma unroll
             for (int w = 0; w < WARPS; w++) total += part[w][threadIdx.x];
             factor[threadIdx.x] = 1.0 / sqrt(total / static_cast<double>(C) + a.eps);
-        }
+            return total;
+        };
         __syncthreads();
-        double r[4];
-        bool fast = true;
+        double total = 0.0;
+        if (threadIdx.x < CODE_BLOCK) total = put_factor();
+        if (sizeof(Sum<T>) == 8) __syncthreads();
+        else if (__syncthreads_or(out_of_range(total, 0.0, a.eps)))
+        {
+            double again[4] = {};
+            for (int i0 = 0; i0 < own; i0 += HELD)
+            {
+                if (!held) load(a.residual != nullptr ? a.sum : a.x, i0, s);
+                add_squares(s, again);
+            }
+            put_sums(again);
+            __syncthreads();
+            if (threadIdx.x < CODE_BLOCK) put_factor();
+            __syncthreads();
+        }
+        Factor<T> r[4];
+        bool all_ordinary = true;
 #pragma unroll
         for (int k = 0; k < 4; k++)
         {
-            r[k] = factor[quad_at<VEC>(lane, k)];
-            fast = fast && ordinary(r[k]);
+            const double v = factor[quad_at<VEC>(lane, k)];
+            r[k].set(v);
+            all_ordinary = all_ordinary && ordinary(v);
         }
-        fast = __all_sync(0xffffffffu, fast);
-        const T* again = static_cast<const T*>(a.residual != nullptr ? a.sum : a.x);
-        for (int64_t c0 = warp; c0 < C; c0 += HELD * WARPS)
+        all_ordinary = __all_sync(0xffffffffu, all_ordinary);
+        for (int i0 = 0; i0 < own; i0 += HELD)
         {
-            if (!held)
+            if (!held) load(a.residual != nullptr ? a.sum : a.x, i0, s);
 #pragma unroll
-                for (int i = 0; i < HELD; i++)
-                {
-                    const int64_t c = c0 + i * WARPS;
-                    s[i] = load_quad<VEC>(again + first + c * a.inner, lane, c < C ? valid : 0);
-                }
-#pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int g0 = 0; g0 < HELD; g0 += GROUP)
             {
-                const int64_t c = c0 + i * WARPS;
-                if (c >= C) continue;
-                const Wide<T> weight = a.weight == nullptr ? Wide<T>(1) : widen(static_cast<const T*>(a.weight)[c]);
-                const Wide<T> g[4] = {weight, weight, weight, weight};
-                put_result<VEC>(a, s[i], r, g, fast, first + c * a.inner, first_block + c * a.tiles_per_row, lane, valid);
+                const int at = i0 + g0;
+                if (at >= own) break;
+                const int lefts[GROUP] = {left, at + 1 < own ? left : 0, at + 2 < own ? left : 0, at + 3 < own ? left : 0};
+                W g[GROUP];
+                bool usual = all_ordinary;
+#pragma unroll
+                for (int i = 0; i < GROUP; i++)
+                {
+                    g[i] = a.weight == nullptr || at + i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[warp + (at + i) * WARPS]);
+                    usual = usual && ordinary_weight(g[i]);
+                }
+                Quad<T> y[GROUP];
+#pragma unroll
+                for (int i = 0; i < GROUP; i++)
+                {
+                    W v[4], result[4];
+                    widen_quad(s[g0 + i], v);
+                    const W weights[4] = {g[i], g[i], g[i], g[i]};
+                    if (usual) times(v, r[0], r[1], r[2], r[3], weights, result);
+                    else
+                    {
+                        rarely();
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            result[k] = static_cast<W>(static_cast<double>(v[k]) * factor[quad_at<VEC>(lane, k)] * static_cast<double>(g[i]));
+                    }
+                    y[i] = narrow_quad<T>(result);
+                }
+                if (a.y != nullptr)
+                {
+                    T* p = static_cast<T*>(a.y) + first + at * step;
+#pragma unroll
+                    for (int i = 0; i < GROUP; i++, p += step) store_quad<VEC>(p, y[i], lefts[i]);
+                }
+                if (a.y_codes != nullptr)
+                    put_codes<VEC>(a.y_codes + first + at * step, static_cast<W*>(a.y_scales) + first_block + at * block_step, step, block_step, y, own - at, lane,
+                                   lefts);
             }
         }
     }
@@ -214,47 +317,94 @@ template <int WARPS> __device__ __forceinline__ double group_sum(double v, doubl
 
 /// Forward, rows of channels: `per_row` warps (a power of two) take a row, warp w of them the blocks w, w + per_row, ... of 128
 /// channels, at most HELD of them.
-template <typename T, bool VEC, int HELD, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) rms_norm_rows_kernel(const NormArgs a, int per_row)
+template <typename T, bool VEC, int HELD, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int per_row)
 {
+    static_assert(HELD % GROUP == 0, "whole groups");
+    using W = Wide<T>;
     __shared__ double part[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % per_row, groups = WARPS / per_row;
-    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row);
+    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row), step = per_row * CODE_BLOCK;
+    const int c0 = sub * CODE_BLOCK + lane_at<VEC>(lane);   // the lane's first channel
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < a.outer; row0 += static_cast<int64_t>(gridDim.x) * groups)
     {
-        const int64_t row = row0 + warp / per_row, first = row * C;
-        const bool live = row < a.outer;   // a warp without a row still takes part in the sums
+        const int64_t row = row0 + warp / per_row, first = row * C + c0;
+        const int64_t first_block = row * blocks + sub;
+        const int own = row < a.outer ? (blocks - sub + per_row - 1) / per_row : 0;   // a warp without a row still takes part in the sums
+        // What lies from the lane's element of block i to the end of the block.
+        const auto left_of = [&](int i) { return i < own ? min(CODE_BLOCK - lane_at<VEC>(lane), C - c0 - i * step) : 0; };
         Quad<T> s[HELD];
-        double sums = 0.0;
+        const auto load = [&](const void* from, int64_t at, Quad<T> (&q)[HELD]) {
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
+            for (int i = 0; i < HELD; i++) q[i] = load_quad<VEC>(static_cast<const T*>(from) + at + i * step, left_of(i));
+        };
+        load(a.x, first, s);
+        if (a.residual != nullptr)
         {
-            const int j = sub + i * per_row;
-            s[i] = take_sum<VEC, T>(a, first + j * CODE_BLOCK, lane, live ? present(j, C) : 0);
-        }
+            Quad<T> more[HELD];
+            load(a.residual, first, more);
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
-        {
-            const int j = sub + i * per_row, valid = live ? present(j, C) : 0;
-#pragma unroll
-            for (int k = 0; k < 4; k++) sums = fma(static_cast<double>(widen(s[i].e[k])), static_cast<double>(widen(s[i].e[k])), sums);
-            if (valid <= 0) continue;
-            const int64_t at = first + j * CODE_BLOCK;
-            if (a.residual != nullptr) store_quad<VEC>(static_cast<T*>(a.sum) + at, s[i], lane, valid);
-            if (a.sum_codes != nullptr) put_codes<VEC>(a.sum_codes, a.sum_scales, at, row * blocks + j, s[i], lane, valid);
+            for (int i = 0; i < HELD; i++)
+            {
+                s[i] = add_quads(s[i], more[i]);
+                store_quad<VEC>(static_cast<T*>(a.sum) + first + i * step, s[i], left_of(i));
+            }
         }
+        Sum<T> sums[1] = {};
+        add_squares(s, sums);
+        const auto put = [&](int8_t* codes, void* scales, const Quad<T> (&q)[GROUP], int g0) {
+            const int lefts[GROUP] = {left_of(g0), left_of(g0 + 1), left_of(g0 + 2), left_of(g0 + 3)};
+            put_codes<VEC>(codes + first + g0 * step, static_cast<W*>(scales) + first_block + g0 * per_row, step, per_row, q, own - g0, lane, lefts);
+        };
+        if (a.sum_codes != nullptr)
+#pragma unroll
+            for (int g0 = 0; g0 < HELD; g0 += GROUP)
+            {
+                if (g0 >= own) break;
+                const Quad<T> q[GROUP] = {s[g0], s[g0 + 1], s[g0 + 2], s[g0 + 3]};
+                put(a.sum_codes, a.sum_scales, q, g0);
+            }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
-        const double factor = 1.0 / sqrt(group_sum<WARPS>(sums, part, per_row) / static_cast<double>(C) + a.eps);
-        const bool fast = ordinary(factor);
-        const double r[4] = {factor, factor, factor, factor};
-#pragma unroll
-        for (int i = 0; i < HELD; i++)
+        double total = group_sum<WARPS>(static_cast<double>(sums[0]), part, per_row);
+        if (sizeof(Sum<T>) == 4)
         {
-            const int j = sub + i * per_row, valid = live ? present(j, C) : 0;
-            if (valid <= 0) continue;
-            Wide<T> g[4] = {1, 1, 1, 1};
-            if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + j * CODE_BLOCK, lane, valid), g);
-            put_result<VEC>(a, s[i], r, g, fast, first + j * CODE_BLOCK, row * blocks + j, lane, valid);
+            // Squares that left the range of float, or would where eps does not cover them: in double. The warps of a row agree; where
+            // rows are shared the thread block decides as one, because its barriers are in common.
+            bool again = out_of_range(total, 0.0, a.eps);
+            if (per_row > 1) again = __syncthreads_or(again);
+            if (again)
+            {
+                double exact[1] = {};
+                add_squares(s, exact);
+                total = group_sum<WARPS>(exact[0], part, per_row);
+            }
+        }
+        const double factor = 1.0 / sqrt(total / static_cast<double>(C) + a.eps);
+        Factor<T> r;
+        r.set(factor);
+#pragma unroll
+        for (int g0 = 0; g0 < HELD; g0 += GROUP)
+        {
+            if (g0 >= own) break;
+            Quad<T> y[GROUP];
+#pragma unroll
+            for (int i = 0; i < GROUP; i++)
+            {
+                W v[4], g[4] = {1, 1, 1, 1}, result[4];
+                widen_quad(s[g0 + i], v);
+                if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + c0 + (g0 + i) * step, left_of(g0 + i)), g);
+                if (ordinary(factor) && ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]))
+                    times(v, r, r, r, r, g, result);
+                else
+                {
+                    rarely();
+#pragma unroll
+                    for (int k = 0; k < 4; k++) result[k] = static_cast<W>(static_cast<double>(v[k]) * factor * static_cast<double>(g[k]));
+                }
+                y[i] = narrow_quad<T>(result);
+                if (a.y != nullptr) store_quad<VEC>(static_cast<T*>(a.y) + first + (g0 + i) * step, y[i], left_of(g0 + i));
+            }
+            if (a.y_codes != nullptr) put(a.y_codes, a.y_scales, y, g0);
         }
     }
 }
@@ -263,22 +413,26 @@ __global__ void __launch_bounds__(WARPS * 32) rms_norm_rows_kernel(const NormArg
 template <typename T, bool CODES> struct HeldSum
 {
     Quad<T> q;
-    template <bool VEC> __device__ __forceinline__ void load(const NormGradArgs& a, int64_t at, int64_t, int lane, int valid)
+    template <bool VEC> __device__ __forceinline__ void load(const NormGradArgs& a, int64_t at, int64_t, int left, bool)
     {
-        q = load_quad<VEC>(static_cast<const T*>(a.sum) + at, lane, valid);
+        q = load_quad<VEC>(static_cast<const T*>(a.sum) + at, left);
     }
-    __device__ __forceinline__ Wide<T> value(int k) const { return widen(q.e[k]); }
+    __device__ __forceinline__ void values(Wide<T> (&v)[4]) const { widen_quad(q, v); }
 };
 template <typename T> struct HeldSum<T, true>
 {
     uint32_t codes;
     Wide<T> scale;
-    template <bool VEC> __device__ __forceinline__ void load(const NormGradArgs& a, int64_t at, int64_t block, int lane, int valid)
+    template <bool VEC> __device__ __forceinline__ void load(const NormGradArgs& a, int64_t at, int64_t block, int left, bool exists)
     {
-        codes = load_codes<VEC>(a.sum_codes + at, lane, valid);
-        scale = valid > 0 ? __ldg(static_cast<const Wide<T>*>(a.sum_scales) + block) : Wide<T>(0);
+        codes = load_codes<VEC>(a.sum_codes + at, left);
+        scale = exists ? __ldg(static_cast<const Wide<T>*>(a.sum_scales) + block) : Wide<T>(0);
     }
-    __device__ __forceinline__ Wide<T> value(int k) const { return widen(narrow<T>(decode_code(codes, k, scale))); }
+    __device__ __forceinline__ void values(Wide<T> (&v)[4]) const
+    {
+        decode_quad(codes, scale, v);
+        if constexpr (sizeof(T) == 2) widen_quad(narrow_quad<T>(v), v);
+    }
 };
 
 /// The two numbers that a pixel's gradients need from its sums over the channels.
@@ -289,90 +443,107 @@ template <typename W> __device__ __forceinline__ void gradient_factors(double sq
     pull = static_cast<W>(factor * factor * (products / channels));
 }
 
-/// gx of a lane's quad.
-template <bool VEC, typename T>
-__device__ __forceinline__ void put_gradient(const NormGradArgs& a, const Wide<T> (&gx)[4], int64_t at, int lane, int valid)
+/// gx of a lane's quad, `more` being the gradient that comes past the norm.
+template <bool VEC, typename T> __device__ __forceinline__ void put_gradient(const NormGradArgs& a, Wide<T> (&gx)[4], const Quad<T>& more, int64_t at, int left)
 {
-    Quad<T> q;
-    Wide<T> more[4] = {0, 0, 0, 0};
-    if (a.gsum != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.gsum) + at, lane, valid), more);
+    if (a.gsum != nullptr)
+    {
+        Wide<T> v[4];
+        widen_quad(more, v);
 #pragma unroll
-    for (int k = 0; k < 4; k++) q.e[k] = narrow<T>(gx[k] + more[k]);
-    store_quad<VEC>(static_cast<T*>(a.gx) + at, q, lane, valid);
+        for (int k = 0; k < 4; k++) gx[k] += v[k];
+    }
+    store_quad<VEC>(static_cast<T*>(a.gx) + at, narrow_quad<T>(gx), left);
 }
 
 /// Backward, feature maps: tiles as in the forward kernel. The thread blocks stay and walk over the tiles, so that gweight is
 /// summed in registers over all of a block's tiles and leaves as one row of partial sums, which norm_weight_kernel adds up in a fixed
-/// order. With more channels than are held, the tile is read twice (from L2) and gweight's sums live in shared memory.
-template <typename T, bool VEC, bool CODES, int HELD, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) rms_norm_columns_backward_kernel(const NormGradArgs a)
+/// order. With more channels than are held, the tile is read twice (from L2) and gweight's sums live in shared memory. gsum is read
+/// after the sums over the channels, GROUP channels at a time: two resident thread blocks hide that latency, and holding it from the start
+/// costs more registers than there are.
+template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
-    static_assert(WARPS >= 4, "a thread for every pixel of the tile");
+    static_assert(WARPS >= 4 && HELD % GROUP == 0, "a thread for every pixel of the tile");
     __shared__ double part[2][WARPS][CODE_BLOCK];
     __shared__ W factors[2][CODE_BLOCK];
     extern __shared__ __align__(16) unsigned char more_shared[];
     W* const weight_sums = reinterpret_cast<W*>(more_shared);   // [channels], only where the channels are not held
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t C = a.channels;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, C = static_cast<int>(a.channels);
+    const int own = (C - warp + WARPS - 1) / WARPS;   // channels of this warp
     const bool held = C <= HELD * WARPS;
+    const int64_t step = WARPS * a.inner, block_step = WARPS * a.tiles_per_row;
     W weight_sum[HELD] = {};
     if (!held && a.gweight != nullptr)
-        for (int64_t c = threadIdx.x; c < C; c += WARPS * 32) weight_sums[c] = W(0);
+        for (int c = threadIdx.x; c < C; c += WARPS * 32) weight_sums[c] = W(0);
+    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[warp + i * WARPS]); };
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
         const int64_t image = tile / a.tiles_per_row, piece = tile - image * a.tiles_per_row;
-        const int valid = static_cast<int>(min(static_cast<int64_t>(CODE_BLOCK), a.inner - piece * CODE_BLOCK));
-        const int64_t first = image * C * a.inner + piece * CODE_BLOCK, first_block = image * C * a.tiles_per_row + piece;
+        const int left = static_cast<int>(min(static_cast<int64_t>(CODE_BLOCK), a.inner - piece * CODE_BLOCK)) - lane_at<VEC>(lane);
+        const int64_t first = (image * C + warp) * a.inner + piece * CODE_BLOCK + lane_at<VEC>(lane);
+        const int64_t first_block = (image * C + warp) * a.tiles_per_row + piece;
         HeldSum<T, CODES> s[HELD];
         Quad<T> gy[HELD];
-        const auto load = [&](int64_t c0) {
+        const auto load = [&](int i0) {
+            int64_t at = first + i0 * step, block = first_block + i0 * block_step;
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int i = 0; i < HELD; i++, at += step, block += block_step)
             {
-                const int64_t c = c0 + i * WARPS, at = first + c * a.inner;
-                const int present = c < C ? valid : 0;
-                s[i].template load<VEC>(a, at, first_block + c * a.tiles_per_row, lane, present);
-                gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + at, lane, present);
+                s[i].template load<VEC>(a, at, block, i0 + i < own ? left : 0, i0 + i < own);
+                gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + at, i0 + i < own ? left : 0);
             }
         };
-        const auto weight_of = [&](int64_t c) { return a.weight == nullptr || c >= C ? W(1) : widen(static_cast<const T*>(a.weight)[c]); };
-        double squares[4] = {}, products[4] = {};
-        for (int64_t c0 = warp; c0 < C; c0 += HELD * WARPS)
-        {
-            load(c0);
-#pragma unroll
-            for (int i = 0; i < HELD; i++)
+        // Sums over the channels, in the type of `zero`, into part; then, for a thread's pixel, their total.
+        const auto add_up = [&](auto zero, double (&total)[2]) {
+            using A = decltype(zero);
+            A squares[4] = {}, products[4] = {};
+            for (int i0 = 0; i0 < own; i0 += HELD)
             {
-                const W g = weight_of(c0 + i * WARPS);
+                if (!held) load(i0);
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                for (int i = 0; i < HELD; i++)
                 {
-                    const double v = static_cast<double>(s[i].value(k));
-                    squares[k] = fma(v, v, squares[k]);
-                    products[k] = fma(v, static_cast<double>(widen(gy[i].e[k]) * g), products[k]);
+                    const A g = static_cast<A>(weight_of(i0 + i));
+                    W v[4], up[4];
+                    s[i].values(v);
+                    widen_quad(gy[i], up);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        squares[k] = fma(static_cast<A>(v[k]), static_cast<A>(v[k]), squares[k]);
+                        products[k] = fma(static_cast<A>(v[k]), static_cast<A>(up[k]) * g, products[k]);
+                    }
                 }
             }
-        }
 #pragma unroll
-        for (int k = 0; k < 4; k++)
-        {
-            part[0][warp][quad_at<VEC>(lane, k)] = squares[k];
-            part[1][warp][quad_at<VEC>(lane, k)] = products[k];
-        }
-        __syncthreads();
-        if (threadIdx.x < CODE_BLOCK)
-        {
-            double total[2] = {};
-#pragma unroll
-            for (int w = 0; w < WARPS; w++)
+            for (int k = 0; k < 4; k++)
             {
-                total[0] += part[0][w][threadIdx.x];
-                total[1] += part[1][w][threadIdx.x];
+                part[0][warp][quad_at<VEC>(lane, k)] = static_cast<double>(squares[k]);
+                part[1][warp][quad_at<VEC>(lane, k)] = static_cast<double>(products[k]);
             }
-            gradient_factors(total[0], total[1], static_cast<double>(C), a.eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+            __syncthreads();
+            if (threadIdx.x < CODE_BLOCK)
+            {
+#pragma unroll
+                for (int w = 0; w < WARPS; w++)
+                {
+                    total[0] += part[0][w][threadIdx.x];
+                    total[1] += part[1][w][threadIdx.x];
+                }
+                gradient_factors(total[0], total[1], static_cast<double>(C), a.eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+            }
+        };
+        if (held) load(0);
+        double total[2] = {};
+        add_up(W(0), total);
+        if (__syncthreads_or(sizeof(W) == 4 && threadIdx.x < CODE_BLOCK && out_of_range(total[0], total[1], a.eps)))
+        {
+            double again[2] = {};
+            add_up(0.0, again);
+            __syncthreads();
         }
-        __syncthreads();
         W r[4], pull[4];
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -380,30 +551,44 @@ __global__ void __launch_bounds__(WARPS * 32) rms_norm_columns_backward_kernel(c
             r[k] = factors[0][quad_at<VEC>(lane, k)];
             pull[k] = factors[1][quad_at<VEC>(lane, k)];
         }
-        for (int64_t c0 = warp; c0 < C; c0 += HELD * WARPS)
+        for (int i0 = 0; i0 < own; i0 += HELD)
         {
-            if (!held) load(c0);
+            if (!held) load(i0);
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int g0 = 0; g0 < HELD; g0 += GROUP)
             {
-                const int64_t c = c0 + i * WARPS;
-                if (c >= C) continue;
-                const W g = weight_of(c);
-                W gx[4], through = 0;
+                if (i0 + g0 >= own) break;
+                const int64_t group = first + (i0 + g0) * step;
+                Quad<T> more[GROUP];
+                if (a.gsum != nullptr)
+                {
+                    const T* p = static_cast<const T*>(a.gsum) + group;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
-                {
-                    const W v = s[i].value(k), up = widen(gy[i].e[k]);
-                    gx[k] = r[k] * (up * g - v * pull[k]);
-                    through += up * (v * r[k]);
+                    for (int i = 0; i < GROUP; i++, p += step) more[i] = load_quad<VEC>(p, i0 + g0 + i < own ? left : 0);
                 }
-                if (held) weight_sum[i] += through;
-                else if (a.gweight != nullptr)
+                int64_t at = group;
+#pragma unroll
+                for (int i = 0; i < GROUP; i++, at += step)
                 {
-                    through = warp_sum(through);
-                    if (lane == 0) weight_sums[c] += through;   // channel c belongs to this warp alone
+                    const int h = g0 + i;
+                    const W g = weight_of(i0 + h);
+                    W v[4], up[4], gx[4], through = 0;
+                    s[h].values(v);
+                    widen_quad(gy[h], up);
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                    {
+                        gx[k] = r[k] * (up[k] * g - v[k] * pull[k]);
+                        through += up[k] * (v[k] * r[k]);
+                    }
+                    if (held) weight_sum[h] += through;
+                    else if (a.gweight != nullptr)
+                    {
+                        through = warp_sum(through);
+                        if (lane == 0 && i0 + h < own) weight_sums[warp + (i0 + h) * WARPS] += through;   // the channel belongs to this warp alone
+                    }
+                    put_gradient<VEC, T>(a, gx, more[i], at, i0 + h < own ? left : 0);
                 }
-                put_gradient<VEC, T>(a, gx, first + c * a.inner, lane, valid);
             }
         }
     }
@@ -414,83 +599,100 @@ __global__ void __launch_bounds__(WARPS * 32) rms_norm_columns_backward_kernel(c
 #pragma unroll
         for (int i = 0; i < HELD; i++)
         {
-            const int64_t c = warp + i * WARPS;
             const W total = warp_sum(weight_sum[i]);
-            if (lane == 0 && c < C) partial[c] = total;
+            if (lane == 0 && i < own) partial[warp + i * WARPS] = total;
         }
     }
     else
     {
         __syncwarp();
-        for (int64_t c = warp; c < C; c += WARPS)
+        for (int c = warp; c < C; c += WARPS)
             if (lane == 0) partial[c] = weight_sums[c];
     }
 }
 
 /// Backward, rows of channels. gweight's sums stay in the lanes that have the channels; the groups of a thread block add theirs
 /// up in shared memory, one after the other, at the end.
-template <typename T, bool VEC, bool CODES, int HELD, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32) rms_norm_rows_backward_kernel(const NormGradArgs a, int per_row)
+template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kernel(const NormGradArgs a, int per_row)
 {
     using W = Wide<T>;
+    constexpr bool EARLY = HELD * sizeof(W) <= 16;   // gsum is read ahead of the sums where there are registers for it
     __shared__ double part[WARPS];
     extern __shared__ __align__(16) unsigned char more_shared[];
     W* const weight_sums = reinterpret_cast<W*>(more_shared);   // [channels]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % per_row, groups = WARPS / per_row;
-    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row);
+    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row), step = per_row * CODE_BLOCK;
+    const int c0 = sub * CODE_BLOCK + lane_at<VEC>(lane);   // the lane's first channel
+    const int most = (blocks - sub + per_row - 1) / per_row;   // blocks of this warp
     W weight_sum[HELD][4] = {};
     for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < a.outer; row0 += static_cast<int64_t>(gridDim.x) * groups)
     {
-        const int64_t row = row0 + warp / per_row, first = row * C;
-        const bool live = row < a.outer;
+        const int64_t row = row0 + warp / per_row, first = row * C + c0;
+        const int own = row < a.outer ? most : 0;
+        const auto left_of = [&](int i, int n) { return i < n ? min(CODE_BLOCK - lane_at<VEC>(lane), C - c0 - i * step) : 0; };
         HeldSum<T, CODES> s[HELD];
-        Quad<T> gy[HELD];
+        Quad<T> gy[HELD], more[HELD];
 #pragma unroll
         for (int i = 0; i < HELD; i++)
         {
-            const int j = sub + i * per_row, valid = live ? present(j, C) : 0;
-            s[i].template load<VEC>(a, first + j * CODE_BLOCK, row * blocks + j, lane, valid);
-            gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + first + j * CODE_BLOCK, lane, valid);
+            s[i].template load<VEC>(a, first + i * step, row * blocks + sub + i * per_row, left_of(i, own), i < own);
+            gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + first + i * step, left_of(i, own));
         }
-        const auto weights_of = [&](int j, W (&g)[4]) {
-            if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + j * CODE_BLOCK, lane, present(j, C)), g);
+        const auto load_more = [&](int i) { more[i] = load_quad<VEC>(static_cast<const T*>(a.gsum) + first + i * step, left_of(i, own)); };
+        if (EARLY && a.gsum != nullptr)
+#pragma unroll
+            for (int i = 0; i < HELD; i++) load_more(i);
+        const auto weights_of = [&](int i, W (&g)[4]) {
+            if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + c0 + i * step, left_of(i, most)), g);
             else
 #pragma unroll
                 for (int k = 0; k < 4; k++) g[k] = W(1);
         };
-        double squares = 0.0, products = 0.0;
+        const auto add_up = [&](auto zero, double (&total)[2]) {
+            using A = decltype(zero);
+            A squares = 0, products = 0;
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
-        {
-            W g[4];
-            weights_of(sub + i * per_row, g);
-#pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int i = 0; i < HELD; i++)
             {
-                const double v = static_cast<double>(s[i].value(k));
-                squares = fma(v, v, squares);
-                products = fma(v, static_cast<double>(widen(gy[i].e[k]) * g[k]), products);
+                W v[4], up[4], g[4];
+                s[i].values(v);
+                widen_quad(gy[i], up);
+                weights_of(i, g);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                {
+                    squares = fma(static_cast<A>(v[k]), static_cast<A>(v[k]), squares);
+                    products = fma(static_cast<A>(v[k]), static_cast<A>(up[k]) * static_cast<A>(g[k]), products);
+                }
             }
-        }
-        squares = group_sum<WARPS>(squares, part, per_row);
-        products = group_sum<WARPS>(products, part, per_row);
+            total[0] = group_sum<WARPS>(static_cast<double>(squares), part, per_row);
+            total[1] = group_sum<WARPS>(static_cast<double>(products), part, per_row);
+        };
+        double total[2];
+        add_up(W(0), total);
+        // The warps of a row agree; where rows are shared the thread block decides as one, because its barriers are in common.
+        bool again = sizeof(W) == 4 && out_of_range(total[0], total[1], a.eps);
+        if (per_row > 1) again = __syncthreads_or(again);
+        if (again) add_up(0.0, total);
         W r, pull;
-        gradient_factors(squares, products, static_cast<double>(C), a.eps, r, pull);
+        gradient_factors(total[0], total[1], static_cast<double>(C), a.eps, r, pull);
 #pragma unroll
         for (int i = 0; i < HELD; i++)
         {
-            const int j = sub + i * per_row, valid = live ? present(j, C) : 0;
-            if (valid <= 0) continue;
-            W g[4], gx[4];
-            weights_of(j, g);
+            if (i >= own) break;
+            if (!EARLY && a.gsum != nullptr) load_more(i);
+            W v[4], up[4], g[4], gx[4];
+            s[i].values(v);
+            widen_quad(gy[i], up);
+            weights_of(i, g);
 #pragma unroll
             for (int k = 0; k < 4; k++)
             {
-                const W v = s[i].value(k), up = widen(gy[i].e[k]);
-                gx[k] = r * (up * g[k] - v * pull);
-                weight_sum[i][k] += up * (v * r);
+                gx[k] = r * (up[k] * g[k] - v[k] * pull);
+                weight_sum[i][k] += up[k] * (v[k] * r);
             }
-            put_gradient<VEC, T>(a, gx, first + j * CODE_BLOCK, lane, valid);
+            put_gradient<VEC, T>(a, gx, more[i], first + i * step, left_of(i, own));
         }
     }
     if (a.gweight == nullptr) return;

@@ -19,7 +19,7 @@ inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner
     if (inner != 1)
     {
         const int64_t tiles = outer * code_blocks(inner);
-        return std::min(tiles, SMS * (channels <= 64 ? 3 : 2));
+        return std::min(tiles, SMS * (channels <= 64 ? 2 : 1));
     }
     const int64_t blocks = code_blocks(channels);
     int64_t groups = 8;   // rows that a thread block has at work

@@ -39,14 +39,18 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
     if (rows)
     {
         if (a.tiles_per_row > 32)
-            return launch_norm(rms_norm_rows_kernel<T, VEC, 8, 16>, a.outer, 16, 0, stream, "rms_norm_rows_kernel", a, 16);
+            return launch_norm(rms_norm_rows_kernel<T, VEC, 8, 16, 1>, a.outer, 16, 0, stream, "rms_norm_rows_kernel", a, 16);
         const int per_row = warps_per_row(a.tiles_per_row, 4, 8), groups = 8 / per_row;
-        return launch_norm(rms_norm_rows_kernel<T, VEC, 4, 8>, (a.outer + groups - 1) / groups, 8, 0, stream, "rms_norm_rows_kernel", a, per_row);
+        return launch_norm(rms_norm_rows_kernel<T, VEC, 4, 8, sizeof(T) == 8 ? 2 : 3>, (a.outer + groups - 1) / groups, 8, 0, stream, "rms_norm_rows_kernel", a, per_row);
     }
     const auto columns = [&](auto kernel, int warps) { return launch_norm(kernel, a.tiles, warps, 0, stream, "rms_norm_columns_kernel", a); };
-    if (a.channels <= 32) return columns(rms_norm_columns_kernel<T, VEC, 4, 8>, 8);
-    if (a.channels <= 64) return columns(rms_norm_columns_kernel<T, VEC, 8, 8>, 8);
-    return columns(rms_norm_columns_kernel<T, VEC, 8, 16>, 16);
+    if (a.channels <= 32) return columns(rms_norm_columns_kernel<T, VEC, 4, 8, 2>, 8);
+    if constexpr (sizeof(T) == 8) return columns(rms_norm_columns_kernel<T, VEC, 4, 16, 1>, 16);   // eight quads of doubles do not fit the registers
+    else
+    {
+        if (a.channels <= 64) return columns(rms_norm_columns_kernel<T, VEC, 8, 8, sizeof(T) == 2 ? 3 : 2>, 8);
+        return columns(rms_norm_columns_kernel<T, VEC, 8, 16, sizeof(T) == 2 ? 2 : 1>, 16);
+    }
 }
 
 template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
@@ -56,17 +60,18 @@ template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, 
     int rc;
     if (rows)
         rc = a.tiles_per_row > 32
-                 ? launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 8, 16>, grid, 16, sums, stream, "rms_norm_rows_backward_kernel", a, 16)
-                 : launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 4, 8>, grid, 8, sums, stream, "rms_norm_rows_backward_kernel", a,
+                 ? launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 8, 16, 1>, grid, 16, sums, stream, "rms_norm_rows_backward_kernel", a, 16)
+                 : launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 4, 8, 2>, grid, 8, sums, stream, "rms_norm_rows_backward_kernel", a,
                                warps_per_row(a.tiles_per_row, 4, 8));
     else
     {
         const auto columns = [&](auto kernel, int warps, size_t shared) {
             return launch_norm(kernel, grid, warps, shared, stream, "rms_norm_columns_backward_kernel", a);
         };
-        if (a.channels <= 32) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8>, 8, 0);
-        else if (a.channels <= 64) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8>, 8, 0);
-        else rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16>, 16, a.channels > 128 ? sums : 0);
+        if (a.channels <= 32) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>, 8, 0);
+        else if constexpr (sizeof(T) == 8) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>, 16, a.channels > 64 ? sums : 0);
+        else if (a.channels <= 64) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>, 8, 0);
+        else rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>, 16, a.channels > 128 ? sums : 0);
     }
     if (rc != MC_OK || a.gweight == nullptr) return rc;
     norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), THREADS, 0, stream>>>(static_cast<const Wide<T>*>(a.partial),
