@@ -24,7 +24,7 @@ inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner
     const int64_t blocks = code_blocks(channels);
     int64_t groups = 8;   // rows that a thread block has at work
     while (groups > 1 && blocks * groups > 32) groups /= 2;
-    return std::min((outer + groups - 1) / groups, SMS * (blocks > 32 ? 1 : 3));
+    return std::min((outer + groups - 1) / groups, SMS * (blocks > 32 ? 1 : 2));
 }
 
 }  // namespace mc

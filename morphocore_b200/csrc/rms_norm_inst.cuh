@@ -13,7 +13,7 @@ constexpr int LARGEST_GRID = 0x7fffffff;
 template <typename Kernel, typename Args, typename... More>
 int launch_norm(Kernel kernel, int64_t grid, int warps, size_t shared, cudaStream_t stream, const char* what, const Args& a, More... more)
 {
-    if (shared > 8 * 1024)
+    if (shared > 30 * 1024)   // with what a kernel declares itself, the 48 KiB that need no opt-in
     {
         const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
         if (err != cudaSuccess)
@@ -59,22 +59,32 @@ template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, 
     const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
     int rc;
     if (rows)
-        rc = a.tiles_per_row > 32
-                 ? launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 8, 16, 1>, grid, 16, sums, stream, "rms_norm_rows_backward_kernel", a, 16)
-                 : launch_norm(rms_norm_rows_backward_kernel<T, VEC, CODES, 4, 8, 2>, grid, 8, sums, stream, "rms_norm_rows_backward_kernel", a,
-                               warps_per_row(a.tiles_per_row, 4, 8));
+    {
+        // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
+        const auto run = [&](auto kernel, size_t slots, int warps, int per_row) {
+            return launch_norm(kernel, grid, warps, std::max(slots, sums), stream, "rms_norm_rows_backward_kernel", a, per_row);
+        };
+        constexpr size_t FEW = gradient_slot_bytes<T, CODES>(4, 256), MANY = gradient_slot_bytes<T, CODES>(8, 512);
+        constexpr bool FITS = MANY <= 200 * 1024;
+        rc = a.tiles_per_row > 32 ? run(rms_norm_rows_backward_kernel<T, VEC, CODES, FITS, 8, 16, 1>, FITS ? MANY : 0, 16, 16)
+                                  : run(rms_norm_rows_backward_kernel<T, VEC, CODES, true, 4, 8, 2>, FEW, 8, warps_per_row(a.tiles_per_row, 4, 8));
+    }
     else
     {
-        const auto columns = [&](auto kernel, int warps, size_t shared) {
-            return launch_norm(kernel, grid, warps, shared, stream, "rms_norm_columns_backward_kernel", a);
+        const auto columns = [&](auto kernel, int held, int warps) {
+            return launch_norm(kernel, grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream, "rms_norm_columns_backward_kernel", a);
         };
-        if (a.channels <= 32) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>, 8, 0);
-        else if constexpr (sizeof(T) == 8) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>, 16, a.channels > 64 ? sums : 0);
-        else if (a.channels <= 64) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>, 8, 0);
-        else rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>, 16, a.channels > 128 ? sums : 0);
+        const auto twice = [&](auto kernel) { return launch_norm(kernel, grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a); };
+        if (a.channels <= 32) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>, 4, 8);
+        else if constexpr (sizeof(T) == 8)
+            rc = a.channels <= 64 ? columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>, 4, 16)
+                                  : twice(rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>);
+        else if (a.channels <= 64) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>, 8, 8);
+        else if (a.channels <= 128) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>, 8, 16);
+        else rc = twice(rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>);
     }
     if (rc != MC_OK || a.gweight == nullptr) return rc;
-    norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), THREADS, 0, stream>>>(static_cast<const Wide<T>*>(a.partial),
+    norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(static_cast<const Wide<T>*>(a.partial),
                                                                                                 static_cast<T*>(a.gweight), a.channels, static_cast<int>(grid));
     return check_launch("norm_weight_kernel");
 }
