@@ -192,6 +192,18 @@ typedef struct mc_rows_desc
 int mc_encode8(const mc_rows_desc* desc, const void* x, int8_t* codes, void* scales, void* stream);
 int mc_decode8(const mc_rows_desc* desc, const int8_t* codes, const void* scales, void* x, void* stream);
 
+/* Per-channel dilation / erosion (MC_MERGE_IDENTITY) with its input kept in 8 bits, each way in one pass over memory:
+ * mc_morpho_forward's y together with mc_encode8's codes and scales of x (rows of H * W elements), and the gradients of
+ * mc_morpho_backward at the values that the codes stand for, without decoding them first. Results of the forward function are
+ * bit-identical to the two calls it replaces; those of the backward function do not depend on the order in which the hardware
+ * runs the thread blocks. Cover float, 3 x 3 and 5 x 5 structuring elements (per-sample ones too) and widths that are a
+ * multiple of four up to 4096; every other case, MC_FLAG_ACCUMULATE among them, returns MC_ERR_UNSUPPORTED with nothing launched: make the
+ * separate calls. */
+int mc_morpho_forward8(const mc_desc* desc, const void* x, const void* w, void* y, int8_t* codes, void* scales, void* stream);
+size_t mc_morpho_backward8_workspace_bytes(const mc_desc* desc);
+int mc_morpho_backward8(const mc_desc* desc, const int8_t* codes, const void* scales, const void* w, const void* gy, void* gx, void* gw, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
 /* ---- Root-mean-square norm (no counterpart in the reference) ------------------------------------------------------------
  *
  * Tensors are [outer, channels, inner], contiguous: (N, C, H * W) for feature maps, (tokens, C, 1) for rows of channels. With

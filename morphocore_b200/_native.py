@@ -24,6 +24,7 @@ lib.mc_selftest_wait_timeout.argtypes = [ctypes.c_uint64, ctypes.c_void_p]
 lib.mc_morpho_backward_workspace_bytes.restype = ctypes.c_size_t
 lib.mc_smorph_backward_workspace_bytes.restype = ctypes.c_size_t
 lib.mc_smorph_scm_backward_workspace_bytes.restype = ctypes.c_size_t
+lib.mc_morpho_backward8_workspace_bytes.restype = ctypes.c_size_t
 lib.mc_rms_norm_backward_workspace_bytes.restype = ctypes.c_size_t
 torch.ops.load_library(EXT_PATH)
 ops = torch.ops.morphocore

@@ -137,14 +137,20 @@ mc_rows_desc rows_desc(const torch::Tensor& t, int64_t leading, int dtype)
     return d;
 }
 
+/// Room for the 8-bit form of a tensor whose last `row_dims` dimensions make up a row.
+Packed packed_like(const torch::Tensor& t, int64_t row_dims)
+{
+    const int64_t leading = t.dim() - row_dims;
+    std::vector<int64_t> shape = t.sizes().slice(0, leading).vec();
+    shape.push_back(code_blocks(product(t.sizes().slice(leading))));
+    return {at::empty(t.sizes(), t.options().dtype(torch::kChar)), at::empty(shape, t.options().dtype(scale_type_of(t.scalar_type())))};
+}
+
 Packed encoded(const torch::Tensor& x, int64_t row_dims)
 {
     const torch::Tensor t = x.contiguous();
-    const int64_t leading = t.dim() - row_dims;
-    const mc_rows_desc d = rows_desc(t, leading, storage_dtype_of(t));
-    std::vector<int64_t> shape = t.sizes().slice(0, leading).vec();
-    shape.push_back(code_blocks(d.length));
-    Packed p{at::empty(t.sizes(), t.options().dtype(torch::kChar)), at::empty(shape, t.options().dtype(scale_type_of(t.scalar_type())))};
+    const mc_rows_desc d = rows_desc(t, t.dim() - row_dims, storage_dtype_of(t));
+    const Packed p = packed_like(t, row_dims);
     const TraceRange trace("morphocore::encode8");
     check_status(mc_encode8(&d, t.data_ptr(), p.codes.data_ptr<int8_t>(), p.scales.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
     return p;
@@ -239,8 +245,10 @@ struct MorphoCall
     torch::Tensor input4d, weight4d, sample_weight, indices, output;
 };
 
+/// `packed`, where given, receives the 8-bit form of the input if the forward pass can write it on its way (mc_morpho_forward8), and is left
+/// undefined otherwise.
 MorphoCall run_morpho_forward(const torch::Tensor& input, const torch::Tensor& weight, int64_t op, int64_t merge, int64_t padding, double padding_value,
-                              bool save_indices, double noise_scale, int64_t flags)
+                              bool save_indices, double noise_scale, int64_t flags, Packed* packed = nullptr)
 {
     TORCH_CHECK(noise_scale >= 0.0, "noise_scale must be non negative");
     MorphoCall call;
@@ -285,9 +293,39 @@ MorphoCall run_morpho_forward(const torch::Tensor& input, const torch::Tensor& w
         call.indices = at::empty(call.output.sizes(), input4d.options().dtype(torch::kInt));
 
     const TraceRange trace("morphocore::morpho_forward");
+    if (packed != nullptr && identity && d.dtype == MC_F32 && static_cast<int64_t>(d.H) * d.W > 1)
+    {
+        const Packed room = packed_like(input4d, 2);
+        const int rc = mc_morpho_forward8(&d, input4d.data_ptr(), kernel_weight.data_ptr(), call.output.data_ptr(), room.codes.data_ptr<int8_t>(),
+                                          room.scales.data_ptr(), at::cuda::getCurrentCUDAStream().stream());
+        if (rc != MC_ERR_UNSUPPORTED)
+        {
+            check_status(rc);
+            *packed = room;
+            return call;
+        }
+    }
     check_status(mc_morpho_forward(&d, input4d.data_ptr(), kernel_weight.data_ptr(), call.output.data_ptr(),
                                    call.indices.defined() ? call.indices.data_ptr<int32_t>() : nullptr, at::cuda::getCurrentCUDAStream().stream()));
     return call;
+}
+
+/// The backward pass of a per-channel layer straight from its input's codes, where a kernel covers it; false where none does.
+bool identity_backward_8bit(const mc_desc& d, const torch::Tensor& codes, const torch::Tensor& scales, const torch::Tensor& kernel_weight,
+                            const torch::Tensor& grad_output, const torch::Tensor& grad_input, const torch::Tensor& grad_weight)
+{
+    if (!codes.defined() || d.merge != MC_MERGE_IDENTITY || d.dtype != MC_F32) return false;
+    // The kernel wants a row of codes a plane; a caller's own may be others.
+    if (scales.dim() < 1 || scales.size(-1) != code_blocks(static_cast<int64_t>(d.H) * d.W) || scales.numel() != static_cast<int64_t>(d.B) * d.Ci * scales.size(-1))
+        return false;
+    const size_t ws_bytes = mc_morpho_backward8_workspace_bytes(&d);
+    if (ws_bytes == 0) return false;
+    const torch::Tensor workspace = at::empty({static_cast<int64_t>(ws_bytes)}, grad_output.options().dtype(torch::kByte));
+    const int rc = mc_morpho_backward8(&d, codes.data_ptr<int8_t>(), scales.data_ptr(), kernel_weight.data_ptr(), grad_output.data_ptr(),
+                                       grad_input.data_ptr(), grad_weight.data_ptr(), workspace.data_ptr(), ws_bytes, at::cuda::getCurrentCUDAStream().stream());
+    if (rc == MC_ERR_UNSUPPORTED) return false;
+    check_status(rc);
+    return true;
 }
 
 class MorphoFunction : public torch::autograd::Function<MorphoFunction>
@@ -296,13 +334,14 @@ public:
     static torch::Tensor forward(torch::autograd::AutogradContext* ctx, torch::Tensor input, torch::Tensor weight, int64_t op, int64_t merge,
                                  int64_t padding, double padding_value, bool save_indices, double noise_scale, int64_t flags, const Keep& keep)
     {
-        MorphoCall call = run_morpho_forward(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags);
+        Packed packed;
+        MorphoCall call = run_morpho_forward(input, weight, op, merge, padding, padding_value, save_indices, noise_scale, flags,
+                                             keep.in8 && !keep.packed.defined() ? &packed : nullptr);
         // Erosion's structuring element is saved as a copy (the reference saves the flipped one), so that a program may go on
         // to change the parameter in place before the backward pass.
         if ((flags & MC_FLAG_FLIPPED_WEIGHT) != 0 && call.weight4d.is_alias_of(weight)) call.weight4d = call.weight4d.clone();
         // In 8 bits the input is kept as codes, and not at all where the winners are: they are all that the backward pass reads.
-        Packed packed;
-        if (keep.in8 && !call.indices.defined())
+        if (keep.in8 && !packed.defined() && !call.indices.defined())
         {
             const c10::cuda::CUDAGuard device_guard(input.device());
             packed = kept_input(keep, call.input4d);
@@ -354,12 +393,14 @@ public:
         const size_t ws_bytes = mc_morpho_backward_workspace_bytes(&d, have_idx);
         torch::Tensor workspace;
         if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, weight.options().dtype(torch::kByte));
-        const torch::Tensor input = saved[4].defined() ? decoded_input(saved[4], saved[5], weight.scalar_type()) : saved[0];
-
         const TraceRange trace("morphocore::morpho_backward");
-        check_status(mc_morpho_backward(&d, input.defined() ? input.data_ptr() : nullptr, kernel_weight.data_ptr(), have_idx ? indices.data_ptr<int32_t>() : nullptr,
-                                        grad_output.data_ptr(), grad_input.data_ptr(), grad_weight.data_ptr(),
-                                        workspace.defined() ? workspace.data_ptr() : nullptr, ws_bytes, at::cuda::getCurrentCUDAStream().stream()));
+        if (!identity_backward_8bit(d, saved[4], saved[5], kernel_weight, grad_output, grad_input, grad_weight))
+        {
+            const torch::Tensor input = saved[4].defined() ? decoded_input(saved[4], saved[5], weight.scalar_type()) : saved[0];
+            check_status(mc_morpho_backward(&d, input.defined() ? input.data_ptr() : nullptr, kernel_weight.data_ptr(), have_idx ? indices.data_ptr<int32_t>() : nullptr,
+                                            grad_output.data_ptr(), grad_input.data_ptr(), grad_weight.data_ptr(),
+                                            workspace.defined() ? workspace.data_ptr() : nullptr, ws_bytes, at::cuda::getCurrentCUDAStream().stream()));
+        }
 
         grad_input = output_to_original(grad_input, ctx->saved_data["input_dims"].toInt());
         if (ctx->saved_data["weight_dims"].toInt() == 2) grad_weight = grad_weight.squeeze(0).squeeze(0);

@@ -415,3 +415,125 @@ def test_training_step_in_a_graph():
         got = [t.clone() for t in held]
         for a, b in zip(got, step(x.requires_grad_(True), w.detach().requires_grad_(True), alpha.detach().requires_grad_(True))):
             assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+# ---- per-channel layers: the kernels that write and read the codes themselves ---------------------------------------------
+
+PLANES = [(1, 1, 1, 4), (2, 3, 5, 8), (3, 2, 9, 28), (1, 2, 40, 32), (2, 2, 31, 36), (1, 3, 70, 64), (2, 1, 33, 100), (1, 2, 130, 112), (1, 2, 66, 128), (2, 1, 20, 132),
+          (1, 2, 75, 244), (1, 1, 9, 1000), (70, 40, 12, 16), (1, 1, 300, 240)]
+
+
+@pytest.mark.parametrize("k", [3, 5])
+@pytest.mark.parametrize("shape", PLANES, ids=str)
+@pytest.mark.parametrize("op", ["dilation", "erosion"])
+def test_per_channel_layers(op, shape, k):
+    """Strips, runs and column tiles of every kind: the output bit for bit, the input's gradient within the rounding of its sums, of at most
+    k * k terms, the weight's of one sum a lane and row and then of a few in a fixed order."""
+    C = shape[1]
+    x, w, gz = make(shape, torch.float32, 1), make((C, 1, k, k), torch.float32, 2) * 0.1, make(shape, torch.float32, 3)
+    for padding in ("replicate", "geodesic", "constant"):
+        leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)]
+        args = dict(channel_merge_mode="identity", padding_mode=padding, padding_value=0.125)
+        with torch.no_grad():
+            plain = getattr(F, op)(*leaves, **args)
+        z = F.checkpoint_8bit(getattr(F, op), *leaves, **args)
+        assert bool((z == plain).all())
+        got = torch.autograd.grad(z, leaves, gz.cuda())
+        codes, scales, _ = P.encode(x, 2)
+        kept = P.decode(torch.from_numpy(codes), torch.from_numpy(scales), torch.float32)
+        wk = w.numpy() if op == "dilation" else np.ascontiguousarray(w.numpy()[..., ::-1, ::-1])
+        # The oracle in float picks the winners; its sums are taken again in double from them.
+        gx, gw = O.morpho_backward(op, kept.numpy().astype(np.float64), wk.astype(np.float64), gz.numpy().astype(np.float64), "identity", padding, 0.125)
+        gx32, gw32 = O.morpho_backward(op, kept.numpy(), wk, gz.numpy(), "identity", padding, 0.125)
+        gw32 = gw32 if op == "dilation" else gw32[..., ::-1, ::-1]
+        size, size_w = (np.abs(t) for t in O.morpho_backward(op, kept.numpy(), wk, np.abs(gz.numpy()), "identity", padding, 0.125))
+        size_w = size_w if op == "dilation" else size_w[..., ::-1, ::-1]
+        u = 2.0 ** -24
+        assert np.all(np.abs(got[0].cpu().numpy() - gx32) <= 2 * k * k * u * size + 1e-30)
+        # A lane adds up its four columns of up to 64 rows one after the other, then 32 lanes; the oracle, all pixels in float.
+        pixels = shape[0] * shape[2] * shape[3]
+        assert np.all(np.abs(got[1].cpu().numpy() - gw32) <= (256 + 6 + min(pixels, 20000)) * u * size_w + 1e-30)
+        again = torch.autograd.grad(F.checkpoint_8bit(getattr(F, op), *leaves, **args), leaves, gz.cuda())
+        assert all(bool((a == b).all()) for a, b in zip(got, again))
+
+
+@pytest.mark.parametrize("op", ["dilation", "erosion"])
+def test_per_channel_ties_and_masks(op):
+    """Zero structuring elements (every quantised neighbourhood has ties), planes of one value, and pixels without a number."""
+    for seed, shape in enumerate([(2, 3, 17, 40), (1, 2, 12, 260)]):
+        x = make(shape, torch.float32, seed)
+        inf = float("inf")
+        r = torch.rand(shape, generator=torch.Generator().manual_seed(seed))
+        x[:, 0] = torch.round(x[:, 0])
+        x[:, 1][r[:, 1] < 0.3] = -inf
+        x[:, 1][r[:, 1] > 0.8] = inf
+        x[:, -1][r[:, -1] < 0.05] = float("nan")
+        x[0, 0, 3:9] = 2.0
+        x[0, 1, 2:8, 4:30] = -inf if op == "dilation" else inf
+        w = torch.zeros(shape[1], 1, 3, 3)
+        w[-1] = make((1, 3, 3), torch.float32, 5) * 0.1
+        gz = make(shape, torch.float32, 7)
+        leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)]
+        for padding in ("replicate", "geodesic", "zero"):
+            with torch.no_grad():
+                plain = getattr(F, op)(*leaves, "identity", padding)
+            z = F.checkpoint_8bit(getattr(F, op), *leaves, "identity", padding)
+            assert same(z, plain)
+            got = torch.autograd.grad(z, leaves, gz.cuda())
+            kept = F.decode_8bit(F.encode_8bit(x.cuda()))
+            assert bool((kept.isinf() == leaves[0].isinf()).all()) and bool((kept.isnan() == leaves[0].isnan()).all())
+            at = [kept.requires_grad_(True), leaves[1]]
+            want = torch.autograd.grad(getattr(F, op)(*at, "identity", padding), at, gz.cuda())
+            for a, b in zip(got, want):   # the plain layers' kernels, whose atomic sums of a few hundred terms are in float
+                assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+def test_per_channel_noise_uses_each_image_s_weights():
+    x, w = make((3, 2, 11, 20), torch.float32, 1).cuda().requires_grad_(True), (make((2, 1, 5, 5), torch.float32, 2) * 0.1).cuda().requires_grad_(True)
+    g = make((3, 2, 11, 20), torch.float32, 3).cuda()
+    for function in (F.dilation, F.erosion):
+        torch.manual_seed(5)
+        z = F.checkpoint_8bit(function, x, w, "identity", noise_scale=0.5, training=True)
+        torch.manual_seed(5)
+        kept = F.decode_8bit(F.encode_8bit(x.detach())).requires_grad_(True)
+        y = function(kept, w, "identity", noise_scale=0.5, training=True)
+        for a, b in zip(torch.autograd.grad(z, (x, w), g), torch.autograd.grad(y, (kept, w), g)):
+            assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+def test_per_channel_layers_through_the_c_abi():
+    """What the entry points refuse with nothing launched, and an empty batch."""
+    import ctypes
+
+    from _cabi import lib, make_desc, ptr, stream
+    from morphocore_b200 import _native
+    x, w = make((2, 3, 8, 12), torch.float32).cuda(), make((3, 1, 3, 3), torch.float32).cuda()
+    y, codes, scales = torch.empty_like(x), torch.empty(x.shape, dtype=torch.int8, device="cuda"), torch.empty(2, 3, 1, device="cuda")
+    gw = torch.ones(3, 1, 3, 3, device="cuda")
+    before = _native.launch_count()
+
+    def forward(d, x=x, codes=codes):
+        return lib.mc_morpho_forward8(ctypes.byref(d), ptr(x), ptr(w), ptr(y), ptr(codes), ptr(scales), stream())
+
+    def backward(d, need=None):
+        size = lib.mc_morpho_backward8_workspace_bytes(ctypes.byref(d)) if need is None else need
+        ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+        return lib.mc_morpho_backward8(ctypes.byref(d), ptr(codes), ptr(scales), ptr(w), ptr(y), ptr(x), ptr(gw), ptr(ws), ctypes.c_size_t(size), stream())
+
+    good = make_desc("dilation", x, w, "identity")
+    for field, value in (("merge", 2), ("dtype", 1), ("W", 13), ("W", 4100), ("kH", 5), ("kW", 7), ("flags", 2)):
+        d = make_desc("dilation", x, w, "identity")
+        setattr(d, field, value)
+        assert forward(d) == -2 and backward(d) == -2, field
+        assert lib.mc_morpho_backward8_workspace_bytes(ctypes.byref(d)) == 0
+    odd = torch.empty(x.numel() + 1, device="cuda")[1:].view_as(x)
+    assert forward(good, x=odd) == -2 and forward(good, codes=None) == -1 and backward(good, need=0) == -3
+    bad = make_desc("dilation", x, w, "identity")
+    bad.flags = 8
+    assert forward(bad) == -1
+    empty = make_desc("dilation", x, w, "identity")
+    empty.B = 0
+    assert forward(empty) == 0
+    assert _native.launch_count() == before
+    assert backward(empty) == 0 and not gw.any()
+    assert forward(good) == 0 and backward(good) == 0 and _native.launch_count() == before + 3
