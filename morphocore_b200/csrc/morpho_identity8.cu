@@ -36,18 +36,25 @@ Identity8Args common(const mc_desc& d)
     return a;
 }
 
-/// Strips of the backward kernel: as long as they can be while there are eight warps of them an SM, at least 8 rows (a strip computes
-/// K - 1 rows of outputs beyond its own).
+/// Strips of the backward kernel. A strip of r rows takes r + K - 1 steps, and the warps of all strips come in waves of what is resident: the strips
+/// of at least 8 rows with the fewest steps in all. ((16, 64, 112, 112) at 3 x 3: three strips a plane, a few more than are resident at once,
+/// took 125 us where two take 78.)
 void set_strips(Identity8Args& a, const mc_desc& d)
 {
     const int64_t planes = static_cast<int64_t>(d.B) * d.Ci;
     a.column_tiles = d.W <= 128 ? 1 : (d.W + strip_columns(d.W) - 1) / strip_columns(d.W);
-    const int64_t columns = planes * a.column_tiles, wanted = 148 * 8 * (32 / strip_lanes(d.W));
-    int64_t strips = std::max<int64_t>(1, (wanted + columns - 1) / columns);
-    strips = std::max<int64_t>(strips, (d.H + 63) / 64);
-    strips = std::min<int64_t>(strips, std::max(1, d.H / 8));
-    a.strip_rows = static_cast<int>((d.H + strips - 1) / strips);
-    a.strips = (d.H + a.strip_rows - 1) / a.strip_rows;
+    const int64_t columns = planes * a.column_tiles, resident = 148 * (d.kH == 3 ? BACKWARD_WARPS_3 : BACKWARD_WARPS_5) * (32 / strip_lanes(d.W));
+    const int extra = d.kH - 1;
+    int64_t best = 0;
+    for (int strips = 1; strips <= std::max(1, d.H / 8); strips++)
+    {
+        const int rows = (d.H + strips - 1) / strips, count = (d.H + rows - 1) / rows;
+        const int64_t cost = (columns * count + resident - 1) / resident * (rows + extra);
+        if (best != 0 && cost >= best) continue;
+        best = cost;
+        a.strip_rows = rows;
+        a.strips = count;
+    }
     a.parts = d.B * a.column_tiles * a.strips;
     a.units = columns * a.strips;
 }
@@ -71,8 +78,8 @@ template <bool IS_MIN> int forward8(const Identity8Args& a, int K, int64_t block
 
 template <bool IS_MIN> int backward8(const Identity8Args& a, int K, int64_t blocks, cudaStream_t stream)
 {
-    const auto kernel = K == 3 ? identity_backward8_kernel<IS_MIN, 3, 5> : identity_backward8_kernel<IS_MIN, 5, 2>;
-    kernel<<<static_cast<unsigned>(blocks), 128, 0, stream>>>(a);
+    const auto kernel = K == 3 ? identity_backward8_kernel<IS_MIN, 3, BACKWARD_WARPS_3> : identity_backward8_kernel<IS_MIN, 5, BACKWARD_WARPS_5>;
+    kernel<<<static_cast<unsigned>(blocks), 32, 0, stream>>>(a);
     return check_launch("identity_backward8_kernel");
 }
 
@@ -103,6 +110,7 @@ int mc_morpho_forward8(const mc_desc* desc, const void* x, const void* w, void* 
     a.codes = codes;
     a.scales = static_cast<float*>(scales);
     a.chunks = (desc->H * desc->W + RUN - 1) / RUN;
+    a.run_step = 4 * THREADS % desc->W;
     const int64_t blocks = planes * a.chunks;
     if (blocks > 0x7fffffff) return MC_ERR_UNSUPPORTED;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -151,7 +159,7 @@ int mc_morpho_backward8(const mc_desc* desc, const int8_t* codes, const void* sc
     a.codes = const_cast<int8_t*>(codes);
     a.scales = const_cast<float*>(static_cast<const float*>(scales));
     a.partial = static_cast<float*>(workspace);
-    const int64_t units_per_block = 4 * (32 / strip_lanes(desc->W)), blocks = (a.units + units_per_block - 1) / units_per_block;
+    const int64_t units_per_block = 32 / strip_lanes(desc->W), blocks = (a.units + units_per_block - 1) / units_per_block;
     if (blocks > 0x7fffffff) return MC_ERR_UNSUPPORTED;
     const bool erosion = desc->op == MC_OP_EROSION;
     const int launched = erosion ? backward8<true>(a, desc->kH, blocks, s) : backward8<false>(a, desc->kH, blocks, s);
