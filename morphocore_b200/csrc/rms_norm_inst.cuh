@@ -1,4 +1,6 @@
 // Instantiates mc::rms_norm_forward<MC_T> and mc::rms_norm_backward<MC_T>; included by rms_norm_f32.cu, _f64, _f16 and _bf16.
+#include <atomic>
+
 #include "rms_norm.cuh"
 #include "rms_norm_api.cuh"
 
@@ -10,19 +12,30 @@ namespace
 
 constexpr int LARGEST_GRID = 0x7fffffff;
 
-template <typename Kernel, typename Args, typename... More>
-int launch_norm(Kernel kernel, int64_t grid, int warps, size_t shared, cudaStream_t stream, const char* what, const Args& a, More... more)
+/// Launches KERNEL, whose shared memory needs an opt-in where it leaves the first 48 KiB with what the kernel declares itself. The opt-in is asked for
+/// once a device (and again for more): it is 1 us of host time.
+template <auto KERNEL, typename Args, typename... More>
+int launch_norm(int64_t grid, int warps, size_t shared, cudaStream_t stream, const char* what, const Args& a, More... more)
 {
-    if (shared > 30 * 1024)   // with what a kernel declares itself, the 48 KiB that need no opt-in
+    if (shared > 30 * 1024)
     {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+        constexpr int MAX_DEVICES = 64;
+        static std::atomic<size_t> allowed[MAX_DEVICES];
+        int device = 0;
+        cudaError_t err = cudaGetDevice(&device);
+        const bool known = err == cudaSuccess && device >= 0 && device < MAX_DEVICES;
+        if (err == cudaSuccess && !(known && allowed[device].load(std::memory_order_relaxed) >= shared))
+        {
+            err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
+            if (err == cudaSuccess && known) allowed[device].store(shared, std::memory_order_relaxed);
+        }
         if (err != cudaSuccess)
         {
             set_last_error("%s: %s", what, cudaGetErrorString(err));
             return MC_ERR_CUDA;
         }
     }
-    kernel<<<static_cast<unsigned>(std::min<int64_t>(grid, LARGEST_GRID)), warps * 32, shared, stream>>>(a, more...);
+    KERNEL<<<static_cast<unsigned>(std::min<int64_t>(grid, LARGEST_GRID)), warps * 32, shared, stream>>>(a, more...);
     return check_launch(what);
 }
 
@@ -36,56 +49,63 @@ int warps_per_row(int64_t blocks, int held, int most)
 
 template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaStream_t stream)
 {
+    constexpr bool WIDE = sizeof(T) == 8, HALF = sizeof(T) == 2;
+    constexpr const char* ROWS = "rms_norm_rows_kernel";
+    constexpr const char* COLUMNS = "rms_norm_columns_kernel";
     if (rows)
     {
-        if (a.tiles_per_row > 32)
-            return launch_norm(rms_norm_rows_kernel<T, VEC, 8, 16, 1>, a.outer, 16, 0, stream, "rms_norm_rows_kernel", a, 16);
+        if (a.tiles_per_row > 32) return launch_norm<rms_norm_rows_kernel<T, VEC, 8, 16, 1>>(a.outer, 16, 0, stream, ROWS, a, 16);
         const int per_row = warps_per_row(a.tiles_per_row, 4, 8), groups = 8 / per_row;
-        return launch_norm(rms_norm_rows_kernel<T, VEC, 4, 8, sizeof(T) == 8 ? 2 : 3>, (a.outer + groups - 1) / groups, 8, 0, stream, "rms_norm_rows_kernel", a, per_row);
+        return launch_norm<rms_norm_rows_kernel<T, VEC, 4, 8, WIDE ? 2 : 3>>((a.outer + groups - 1) / groups, 8, 0, stream, ROWS, a, per_row);
     }
-    const auto columns = [&](auto kernel, int warps) { return launch_norm(kernel, a.tiles, warps, 0, stream, "rms_norm_columns_kernel", a); };
-    if (a.channels <= 32) return columns(rms_norm_columns_kernel<T, VEC, 4, 8, 2>, 8);
-    if constexpr (sizeof(T) == 8) return columns(rms_norm_columns_kernel<T, VEC, 4, 16, 1>, 16);   // eight quads of doubles do not fit the registers
+    if (a.channels <= 32) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 8, 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
+    if constexpr (WIDE) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 16, 1>>(a.tiles, 16, 0, stream, COLUMNS, a);   // eight quads of doubles do not fit
     else
     {
-        if (a.channels <= 64) return columns(rms_norm_columns_kernel<T, VEC, 8, 8, sizeof(T) == 2 ? 3 : 2>, 8);
-        return columns(rms_norm_columns_kernel<T, VEC, 8, 16, sizeof(T) == 2 ? 2 : 1>, 16);
+        if (a.channels <= 64) return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 8, HALF ? 3 : 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
+        return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 16, HALF ? 2 : 1>>(a.tiles, 16, 0, stream, COLUMNS, a);
     }
+}
+
+template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
+{
+    constexpr const char* ROWS = "rms_norm_rows_backward_kernel";
+    constexpr const char* COLUMNS = "rms_norm_columns_backward_kernel";
+    const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
+    constexpr size_t FEW = gradient_slot_bytes<T, CODES>(4, 256);
+    if (rows)
+    {
+        // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
+        constexpr size_t MANY = gradient_slot_bytes<T, CODES>(8, 512);
+        constexpr bool FITS = MANY <= 200 * 1024;
+        if (a.tiles_per_row > 32)
+            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, FITS, 8, 16, 1>>(grid, 16, std::max(FITS ? MANY : 0, sums), stream, ROWS, a, 16);
+        return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, true, 4, 8, 2>>(grid, 8, std::max(FEW, sums), stream, ROWS, a,
+                                                                                       warps_per_row(a.tiles_per_row, 4, 8));
+    }
+    if (a.channels <= 32) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>>(grid, 8, FEW, stream, COLUMNS, a);
+    if constexpr (sizeof(T) == 8)
+    {
+        if (a.channels <= 64)
+            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(4, 512), stream, COLUMNS, a);
+    }
+    else
+    {
+        if (a.channels <= 64)
+            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>>(grid, 8, gradient_slot_bytes<T, CODES>(8, 256), stream, COLUMNS, a);
+        if (a.channels <= 128)
+            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(8, 512), stream, COLUMNS, a);
+    }
+    return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
 }
 
 template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
     const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner);
-    const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
-    int rc;
-    if (rows)
-    {
-        // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
-        const auto run = [&](auto kernel, size_t slots, int warps, int per_row) {
-            return launch_norm(kernel, grid, warps, std::max(slots, sums), stream, "rms_norm_rows_backward_kernel", a, per_row);
-        };
-        constexpr size_t FEW = gradient_slot_bytes<T, CODES>(4, 256), MANY = gradient_slot_bytes<T, CODES>(8, 512);
-        constexpr bool FITS = MANY <= 200 * 1024;
-        rc = a.tiles_per_row > 32 ? run(rms_norm_rows_backward_kernel<T, VEC, CODES, FITS, 8, 16, 1>, FITS ? MANY : 0, 16, 16)
-                                  : run(rms_norm_rows_backward_kernel<T, VEC, CODES, true, 4, 8, 2>, FEW, 8, warps_per_row(a.tiles_per_row, 4, 8));
-    }
-    else
-    {
-        const auto columns = [&](auto kernel, int held, int warps) {
-            return launch_norm(kernel, grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream, "rms_norm_columns_backward_kernel", a);
-        };
-        const auto twice = [&](auto kernel) { return launch_norm(kernel, grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a); };
-        if (a.channels <= 32) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>, 4, 8);
-        else if constexpr (sizeof(T) == 8)
-            rc = a.channels <= 64 ? columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>, 4, 16)
-                                  : twice(rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>);
-        else if (a.channels <= 64) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>, 8, 8);
-        else if (a.channels <= 128) rc = columns(rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>, 8, 16);
-        else rc = twice(rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>);
-    }
+    const int rc = backward_sums<T, VEC, CODES>(a, rows, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
-    norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(static_cast<const Wide<T>*>(a.partial),
-                                                                                                static_cast<T*>(a.gweight), a.channels, static_cast<int>(grid));
+    norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(
+        static_cast<const Wide<T>*>(a.partial), static_cast<T*>(a.gweight), a.channels, static_cast<int>(grid));
     return check_launch("norm_weight_kernel");
 }
 
