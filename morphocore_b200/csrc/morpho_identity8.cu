@@ -39,7 +39,8 @@ Identity8Args common(const mc_desc& d)
 /// Strips of the backward kernel. A strip of r rows takes r + K - 1 steps, and the warps of all strips come in waves of what is resident: the strips
 /// of at least 8 rows with the fewest steps in all. ((16, 64, 112, 112) at 3 x 3: three strips a plane, a few more than are resident at once,
 /// took 125 us where two take 78.)
-void set_strips(Identity8Args& a, const mc_desc& d)
+/// False where there are more of them than can be counted.
+bool set_strips(Identity8Args& a, const mc_desc& d)
 {
     const int64_t planes = static_cast<int64_t>(d.B) * d.Ci;
     a.column_tiles = d.W <= 128 ? 1 : (d.W + strip_columns(d.W) - 1) / strip_columns(d.W);
@@ -55,8 +56,9 @@ void set_strips(Identity8Args& a, const mc_desc& d)
         a.strip_rows = rows;
         a.strips = count;
     }
-    a.parts = d.B * a.column_tiles * a.strips;
     a.units = columns * a.strips;
+    a.parts = static_cast<int>(std::min<int64_t>(a.units / d.Ci, std::numeric_limits<int>::max()));
+    return a.units / d.Ci < std::numeric_limits<int>::max();
 }
 
 /// Validation of what both entry points take.
@@ -121,7 +123,7 @@ size_t mc_morpho_backward8_workspace_bytes(const mc_desc* desc)
 {
     if (checked(desc) != MC_OK || desc->B == 0) return 0;
     Identity8Args a = common(*desc);
-    set_strips(a, *desc);
+    if (!set_strips(a, *desc)) return 0;
     return sizeof(float) * static_cast<size_t>(desc->Ci) * desc->kH * desc->kW * static_cast<size_t>(a.parts);
 }
 
@@ -146,13 +148,14 @@ int mc_morpho_backward8(const mc_desc* desc, const int8_t* codes, const void* sc
     }
     if (!aligned16({gy, gx}) || reinterpret_cast<uintptr_t>(codes) % 4 != 0) return MC_ERR_UNSUPPORTED;
     const size_t need = mc_morpho_backward8_workspace_bytes(desc);
+    if (need == 0) return MC_ERR_UNSUPPORTED;
     if (workspace == nullptr || workspace_bytes < need)
     {
         set_last_error("workspace of %zu bytes needed, %zu given", need, workspace_bytes);
         return MC_ERR_WORKSPACE;
     }
     Identity8Args a = common(*desc);
-    set_strips(a, *desc);
+    (void)set_strips(a, *desc);
     a.w = static_cast<const float*>(w);
     a.gy = static_cast<const float*>(gy);
     a.y = static_cast<float*>(gx);

@@ -286,6 +286,18 @@ def test_empty_and_refusals():
         y.sum().backward()
 
 
+def test_tangents_are_refused():
+    """Forward-mode tangents and functorch transforms have no rule here: they raise instead of being dropped on the way."""
+    import torch.autograd.forward_ad as fwad
+    x, w = torch.randn(2, 4, 5, 6, device="cuda"), torch.ones(4, device="cuda")
+    for call in (lambda t: F.rms_norm(t, w), lambda t: F.rms_norm(x, w, t)[0], lambda t: F.checkpoint_8bit(F.rms_norm, t, w),
+                 lambda t: F.checkpoint_8bit(F.dilation, t, w.expand(3, 4)[:, :, None, None])):
+        with pytest.raises(RuntimeError), fwad.dual_level():
+            call(fwad.make_dual(x, torch.ones_like(x)))
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: call(t).sum())(x)
+
+
 def test_streams_and_graphs():
     """Two replayed graphs and a side stream, forward and backward: each has workspaces of its own."""
     x, r, w, s = cuda(*tensors((4, 70, 20, 21), 1, torch.float32))
