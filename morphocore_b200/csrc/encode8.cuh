@@ -112,13 +112,14 @@ template <typename T> __device__ __forceinline__ Quad<T> narrow_quad(const Wide<
 
 /// Position within the block of a lane's first element; and of element k.
 template <bool VEC> __device__ __forceinline__ int lane_at(int lane) { return VEC ? 4 * lane : lane; }
-template <bool VEC> __device__ __forceinline__ int quad_at(int lane, int k) { return lane_at<VEC>(lane) + (VEC ? k : 32 * k); }
+template <bool VEC, int LANES = 32> __device__ __forceinline__ int quad_at(int lane, int k) { return lane_at<VEC>(lane) + (VEC ? k : LANES * k); }
 
 // The four functions below take the address of the lane's first element and how many elements of the block lie from there on: with
-// VEC all four of a lane exist (left > 0) or none, otherwise element k does where 32 k < left.
+// VEC all four of a lane exist (left > 0) or none, otherwise element k does where 32 k < left. Where LANES lanes share a shorter block, they stand
+// for the 32.
 
 /// A lane's elements; zeros where there are none.
-template <bool VEC, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* src, int left)
+template <bool VEC, int LANES = 32, typename T> __device__ __forceinline__ Quad<T> load_quad(const T* src, int left)
 {
     Quad<T> q{};
     if constexpr (VEC)
@@ -129,17 +130,17 @@ template <bool VEC, typename T> __device__ __forceinline__ Quad<T> load_quad(con
     {
         uint32_t half[4];
 #pragma unroll
-        for (int k = 0; k < 4; k++) half[k] = 32 * k < left ? reinterpret_cast<const uint16_t*>(src)[32 * k] : 0u;
+        for (int k = 0; k < 4; k++) half[k] = LANES * k < left ? reinterpret_cast<const uint16_t*>(src)[LANES * k] : 0u;
 #pragma unroll
         for (int h = 0; h < 2; h++) q.word[h] = half[2 * h] | half[2 * h + 1] << 16;
     }
     else
 #pragma unroll
-        for (int k = 0; k < 4; k++) q.e[k] = 32 * k < left ? src[32 * k] : T(0);
+        for (int k = 0; k < 4; k++) q.e[k] = LANES * k < left ? src[LANES * k] : T(0);
     return q;
 }
 
-template <bool VEC, typename T> __device__ __forceinline__ void store_quad(T* dst, const Quad<T>& q, int left)
+template <bool VEC, int LANES = 32, typename T> __device__ __forceinline__ void store_quad(T* dst, const Quad<T>& q, int left)
 {
     if constexpr (VEC)
     {
@@ -148,15 +149,15 @@ template <bool VEC, typename T> __device__ __forceinline__ void store_quad(T* ds
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (32 * k < left)
+            if (LANES * k < left)
             {
-                if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(dst)[32 * k] = static_cast<uint16_t>(q.word[k / 2] >> (16 * (k % 2)));
-                else dst[32 * k] = q.e[k];
+                if constexpr (sizeof(T) == 2) reinterpret_cast<uint16_t*>(dst)[LANES * k] = static_cast<uint16_t>(q.word[k / 2] >> (16 * (k % 2)));
+                else dst[LANES * k] = q.e[k];
             }
 }
 
 /// A lane's four codes, element k in byte k.
-template <bool VEC> __device__ __forceinline__ uint32_t load_codes(const int8_t* src, int left)
+template <bool VEC, int LANES = 32> __device__ __forceinline__ uint32_t load_codes(const int8_t* src, int left)
 {
     uint32_t q = 0;
     if constexpr (VEC)
@@ -166,11 +167,11 @@ template <bool VEC> __device__ __forceinline__ uint32_t load_codes(const int8_t*
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (32 * k < left) q |= static_cast<uint32_t>(static_cast<uint8_t>(src[32 * k])) << (8 * k);
+            if (LANES * k < left) q |= static_cast<uint32_t>(static_cast<uint8_t>(src[LANES * k])) << (8 * k);
     return q;
 }
 
-template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* dst, uint32_t codes, int left)
+template <bool VEC, int LANES = 32> __device__ __forceinline__ void store_codes(int8_t* dst, uint32_t codes, int left)
 {
     if constexpr (VEC)
     {
@@ -179,7 +180,7 @@ template <bool VEC> __device__ __forceinline__ void store_codes(int8_t* dst, uin
     else
 #pragma unroll
         for (int k = 0; k < 4; k++)
-            if (32 * k < left) dst[32 * k] = static_cast<int8_t>(codes >> (8 * k));
+            if (LANES * k < left) dst[LANES * k] = static_cast<int8_t>(codes >> (8 * k));
 }
 
 __device__ __forceinline__ uint32_t pack_bytes(const uint32_t (&q)[4])

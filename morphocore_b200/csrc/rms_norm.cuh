@@ -104,18 +104,14 @@ __device__ __forceinline__ bool out_of_range(double squares, double products, do
     return !(squares < 0x1p120) || (squares < 0x1p-60 && eps < 0x1p-60) || !(fabs(products) < 0x1p120);
 }
 
-__device__ __forceinline__ double warp_sum(double v)
+/// Sum over LANES neighbouring lanes, the same in each of them.
+template <int LANES, typename V> __device__ __forceinline__ V lanes_sum(V v)
 {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+    for (int d = LANES / 2; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-__device__ __forceinline__ float warp_sum(float v)
-{
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    return v;
-}
+template <typename V> __device__ __forceinline__ V warp_sum(V v) { return lanes_sum<32>(v); }
 
 /// Keeps the compiler from holding the widened elements of a quad of half precision from one use to the next: they are cheaper to make again
 /// than the registers that they fill.
@@ -184,7 +180,7 @@ __device__ __forceinline__ void fetch_commit() { asm volatile("cp.async.commit_g
 template <int PENDING> __device__ __forceinline__ void fetch_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 /// A quad of `base + at` on its way into a slot. Single elements of half precision have no asynchronous copy: they are loaded there and then.
-template <bool VEC, typename T> __device__ __forceinline__ void fetch_quad(Quad<T>* slot, const T* base, int64_t at, int left)
+template <bool VEC, int LANES = 32, typename T> __device__ __forceinline__ void fetch_quad(Quad<T>* slot, const T* base, int64_t at, int left)
 {
     if constexpr (VEC)
     {
@@ -197,14 +193,14 @@ template <bool VEC, typename T> __device__ __forceinline__ void fetch_quad(Quad<
     else if constexpr (sizeof(T) >= 4)
     {
 #pragma unroll
-        for (int k = 0; k < 4; k++) fetch_bytes<sizeof(T)>(&slot->e[k], 32 * k < left ? base + at + 32 * k : base, 32 * k < left);
+        for (int k = 0; k < 4; k++) fetch_bytes<sizeof(T)>(&slot->e[k], LANES * k < left ? base + at + LANES * k : base, LANES * k < left);
     }
-    else *slot = load_quad<VEC>(base + at, left);
+    else *slot = load_quad<VEC, LANES>(base + at, left);
 }
-template <bool VEC> __device__ __forceinline__ void fetch_codes(uint32_t* slot, const int8_t* base, int64_t at, int left)
+template <bool VEC, int LANES = 32> __device__ __forceinline__ void fetch_codes(uint32_t* slot, const int8_t* base, int64_t at, int left)
 {
     if constexpr (VEC) fetch_bytes<4>(slot, left > 0 ? base + at : base, left > 0);
-    else *slot = load_codes<VEC>(base + at, left);
+    else *slot = load_codes<VEC, LANES>(base + at, left);
 }
 
 /// Blocks are finished and encoded this many at a time.
@@ -483,9 +479,9 @@ template <typename T, bool CODES> struct HeldSum
         q = load_quad<VEC>(static_cast<const T*>(a.sum) + at, left);
     }
     using Slot = Quad<T>;
-    template <bool VEC> static __device__ __forceinline__ void fetch(const NormGradArgs& a, Slot* slot, int64_t at, int left)
+    template <bool VEC, int LANES = 32> static __device__ __forceinline__ void fetch(const NormGradArgs& a, Slot* slot, int64_t at, int left)
     {
-        fetch_quad<VEC>(slot, static_cast<const T*>(a.sum), at, left);
+        fetch_quad<VEC, LANES>(slot, static_cast<const T*>(a.sum), at, left);
     }
     __device__ __forceinline__ void take(const Slot& slot, Wide<T>) { q = slot; }
     __device__ __forceinline__ void forget_values() { forget_widened(q); }
@@ -501,9 +497,9 @@ template <typename T> struct HeldSum<T, true>
         scale = exists ? __ldg(static_cast<const Wide<T>*>(a.sum_scales) + block) : Wide<T>(0);
     }
     using Slot = uint32_t;
-    template <bool VEC> static __device__ __forceinline__ void fetch(const NormGradArgs& a, Slot* slot, int64_t at, int left)
+    template <bool VEC, int LANES = 32> static __device__ __forceinline__ void fetch(const NormGradArgs& a, Slot* slot, int64_t at, int left)
     {
-        fetch_codes<VEC>(slot, a.sum_codes, at, left);
+        fetch_codes<VEC, LANES>(slot, a.sum_codes, at, left);
     }
     __device__ __forceinline__ void take(const Slot& slot, Wide<T> s)
     {
@@ -527,7 +523,7 @@ template <typename W> __device__ __forceinline__ void gradient_factors(double sq
 }
 
 /// gx of a lane's quad, `more` pointing to the gradient that comes past the norm.
-template <bool VEC, typename T> __device__ __forceinline__ void put_gradient(const NormGradArgs& a, Wide<T> (&gx)[4], const Quad<T>* more, int64_t at, int left)
+template <bool VEC, int LANES, typename T> __device__ __forceinline__ void put_gradient(const NormGradArgs& a, Wide<T> (&gx)[4], const Quad<T>* more, int64_t at, int left)
 {
     if (a.gsum != nullptr)
     {
@@ -536,54 +532,55 @@ template <bool VEC, typename T> __device__ __forceinline__ void put_gradient(con
 #pragma unroll
         for (int k = 0; k < 4; k++) gx[k] += v[k];
     }
-    store_quad<VEC>(static_cast<T*>(a.gx) + at, narrow_quad<T>(gx), left);
+    store_quad<VEC, LANES>(static_cast<T*>(a.gx) + at, narrow_quad<T>(gx), left);
 }
 
 /// The factors of a tile's pixels in the backward kernels, r and the pull of the sum, in shared memory for all threads. `add_up` adds squares and
 /// products of the warp's channels up in the type that it is given, and again in double where float's range was left: squares and products in
 /// turn then, because the room is that of both in float. Ends with a barrier.
-template <bool VEC, typename W, int WARPS, typename AddUp>
-__device__ __forceinline__ void tile_gradient_factors(W (&part)[2][WARPS][CODE_BLOCK], W (&factors)[2][CODE_BLOCK], int C, double eps, int lane, int warp, AddUp add_up)
+template <bool VEC, int LANES, typename W, int GROUPS, int PIXELS, typename AddUp>
+__device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXELS], W (&factors)[2][PIXELS], int C, double eps, int lane, int group, AddUp add_up)
 {
     W sums[2][4] = {};
     add_up(sums);
 #pragma unroll
     for (int k = 0; k < 4; k++)
     {
-        part[0][warp][quad_at<VEC>(lane, k)] = sums[0][k];
-        part[1][warp][quad_at<VEC>(lane, k)] = sums[1][k];
+        part[0][group][quad_at<VEC, LANES>(lane, k)] = sums[0][k];
+        part[1][group][quad_at<VEC, LANES>(lane, k)] = sums[1][k];
     }
     __syncthreads();
     double total[2] = {};
-    if (threadIdx.x < CODE_BLOCK)
+    if (threadIdx.x < PIXELS)
     {
 #pragma unroll
-        for (int w = 0; w < WARPS; w++)
+        for (int g = 0; g < GROUPS; g++)
         {
-            total[0] += static_cast<double>(part[0][w][threadIdx.x]);
-            total[1] += static_cast<double>(part[1][w][threadIdx.x]);
+            total[0] += static_cast<double>(part[0][g][threadIdx.x]);
+            total[1] += static_cast<double>(part[1][g][threadIdx.x]);
         }
         gradient_factors(total[0], total[1], static_cast<double>(C), eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
     }
     if constexpr (sizeof(W) == 8) __syncthreads();
-    else if (__syncthreads_or(threadIdx.x < CODE_BLOCK && out_of_range(total[0], total[1], eps)))
+    else if (__syncthreads_or(threadIdx.x < PIXELS && out_of_range(total[0], total[1], eps)))
     {
+        rarely();
         double exact[2][4] = {};
         add_up(exact);
-        double(*const wide)[CODE_BLOCK] = reinterpret_cast<double(*)[CODE_BLOCK]>(&part[0][0][0]);   // [WARPS][128]
+        double(*const wide)[PIXELS] = reinterpret_cast<double(*)[PIXELS]>(&part[0][0][0]);   // [GROUPS][PIXELS]
         for (int q = 0; q < 2; q++)
         {
 #pragma unroll
-            for (int k = 0; k < 4; k++) wide[warp][quad_at<VEC>(lane, k)] = q == 0 ? exact[0][k] : exact[1][k];
+            for (int k = 0; k < 4; k++) wide[group][quad_at<VEC, LANES>(lane, k)] = q == 0 ? exact[0][k] : exact[1][k];
             __syncthreads();
-            if (threadIdx.x < CODE_BLOCK)
+            if (threadIdx.x < PIXELS)
             {
                 total[q] = 0.0;
-                for (int w = 0; w < WARPS; w++) total[q] += wide[w][threadIdx.x];
+                for (int g = 0; g < GROUPS; g++) total[q] += wide[g][threadIdx.x];
             }
             __syncthreads();
         }
-        if (threadIdx.x < CODE_BLOCK) gradient_factors(total[0], total[1], static_cast<double>(C), eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        if (threadIdx.x < PIXELS) gradient_factors(total[0], total[1], static_cast<double>(C), eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
         __syncthreads();
     }
 }
@@ -619,33 +616,41 @@ template <typename T, bool CODES> constexpr size_t gradient_slot_bytes(int held,
     return (2 * sizeof(Quad<T>) + sizeof(typename HeldSum<T, CODES>::Slot)) * static_cast<size_t>(held) * threads;
 }
 
-/// Backward, feature maps of up to HELD * WARPS channels: tiles, channels and fetching as in the forward kernel. The thread blocks walk over the
-/// tiles with gweight's sums in registers; what they have at the end leaves as one row of partial sums, which norm_weight_kernel adds up in a
-/// fixed order.
-template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int CTAS>
+/// Backward, feature maps of up to HELD * WARPS * SPLIT channels. A tile is 128 / SPLIT pixels of an image; SPLIT groups of lanes of a warp have
+/// channels of their own, so that a thread block of few warps holds many channels and two of them, which hide each other's barriers, stay
+/// resident. Tiles of 32 pixels, read once, against whole ones read twice: (64, 256, 56, 56) 144 us against 170, (64, 512, 28, 28) 97 against
+/// 118; of 64 pixels in thread blocks of 8 warps against whole ones in 16: (16, 128, 112, 112) 78 against 82. The thread blocks walk over the tiles with
+/// gweight's sums in registers; what they have at the end leaves as one row of partial sums, which norm_weight_kernel adds up in a fixed order.
+template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int SPLIT, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
     using Held = HeldSum<T, CODES>;
-    constexpr int COUNT = WARPS * 32;
-    static_assert(WARPS >= 4 && HELD <= 32, "a thread for every pixel of the tile, a lane for every scale");
-    __shared__ W part[2][WARPS][CODE_BLOCK];
-    __shared__ W factors[2][CODE_BLOCK];
+    constexpr int COUNT = WARPS * 32, LANES = 32 / SPLIT, PIXELS = CODE_BLOCK / SPLIT, STEP = WARPS * SPLIT;
+    static_assert(WARPS * 32 >= PIXELS && HELD <= LANES, "a thread for every pixel of the tile, a lane for every scale");
+    __shared__ W part[2][STEP][PIXELS];
+    __shared__ W factors[2][PIXELS];
     extern __shared__ __align__(16) unsigned char slots[];
     Quad<T>* const gy_slot = reinterpret_cast<Quad<T>*>(slots) + threadIdx.x;   // [HELD][threads] each
     Quad<T>* const more_slot = gy_slot + HELD * COUNT;
     typename Held::Slot* const sum_slot = reinterpret_cast<typename Held::Slot*>(slots + 2 * HELD * COUNT * sizeof(Quad<T>)) + threadIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, C = static_cast<int>(a.channels);
-    const int own = (C - warp + WARPS - 1) / WARPS;   // channels of this warp
-    const int64_t step = WARPS * a.inner, block_step = WARPS * a.tiles_per_row;
-    W next_scale = 0;   // lane i: of the warp's channel i
+    const int C = static_cast<int>(a.channels);
+    const int lane = threadIdx.x & (LANES - 1), group = threadIdx.x / LANES;   // the group has the channels group, group + STEP, ...
+    const int own = (C - group + STEP - 1) / STEP;
+    const int64_t step = STEP * a.inner, block_step = STEP * a.tiles_per_row, pieces = (a.inner + PIXELS - 1) / PIXELS, tiles = a.outer * pieces;
+    W next_scale = 0;   // lane i: of the group's channel i
+    const auto place = [&](int64_t tile) {
+        const int64_t image = tile / pieces, pixel = (tile - image * pieces) * PIXELS, row = image * C + group;
+        return Place{row * a.inner + pixel + lane_at<VEC>(lane), row * a.tiles_per_row + pixel / CODE_BLOCK,
+                     static_cast<int>(min(static_cast<int64_t>(PIXELS), a.inner - pixel)) - lane_at<VEC>(lane)};
+    };
     const auto fetch = [&](const Place& p) {
         int64_t at = p.first;
 #pragma unroll
         for (int i = 0; i < HELD; i++, at += step)
         {
-            Held::template fetch<VEC>(a, sum_slot + i * COUNT, at, i < own ? p.left : 0);
-            fetch_quad<VEC>(gy_slot + i * COUNT, static_cast<const T*>(a.gy), at, i < own ? p.left : 0);
+            Held::template fetch<VEC, LANES>(a, sum_slot + i * COUNT, at, i < own ? p.left : 0);
+            fetch_quad<VEC, LANES>(gy_slot + i * COUNT, static_cast<const T*>(a.gy), at, i < own ? p.left : 0);
         }
         if (CODES && lane < min(own, HELD)) next_scale = __ldg(static_cast<const W*>(a.sum_scales) + p.block + lane * block_step);
     };
@@ -653,17 +658,17 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
         if (a.gsum == nullptr) return;
         int64_t at = p.first;
 #pragma unroll
-        for (int i = 0; i < HELD; i++, at += step) fetch_quad<VEC>(more_slot + i * COUNT, static_cast<const T*>(a.gsum), at, i < own ? p.left : 0);
+        for (int i = 0; i < HELD; i++, at += step) fetch_quad<VEC, LANES>(more_slot + i * COUNT, static_cast<const T*>(a.gsum), at, i < own ? p.left : 0);
     };
-    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[warp + i * WARPS]); };
+    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[group + i * STEP]); };
     W weight_sum[HELD] = {};
     int64_t tile = blockIdx.x;
-    Place p = place_of<VEC>(a, tile, lane, warp);
+    Place p = place(tile);
     fetch(p);
     fetch_commit();
     fetch_more(p);
     fetch_commit();
-    for (; tile < a.tiles; tile += gridDim.x)
+    for (; tile < tiles; tile += gridDim.x)
     {
         fetch_wait<1>();   // gsum may still travel
         Held s[HELD];
@@ -671,19 +676,19 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 #pragma unroll
         for (int i = 0; i < HELD; i++)
         {
-            s[i].take(sum_slot[i * COUNT], CODES ? __shfl_sync(0xffffffffu, next_scale, i) : W(0));
+            s[i].take(sum_slot[i * COUNT], CODES ? __shfl_sync(0xffffffffu, next_scale, i, LANES) : W(0));
             gy[i] = gy_slot[i * COUNT];
         }
         __syncwarp();
         const Place here = p;
-        const bool last = tile + gridDim.x >= a.tiles;
+        const bool last = tile + gridDim.x >= tiles;
         if (!last)
         {
-            p = place_of<VEC>(a, tile + gridDim.x, lane, warp);
+            p = place(tile + gridDim.x);
             fetch(p);
         }
         fetch_commit();
-        tile_gradient_factors<VEC>(part, factors, C, a.eps, lane, warp, [&](auto& sums) {
+        tile_gradient_factors<VEC, LANES>(part, factors, C, a.eps, lane, group, [&](auto& sums) {
 #pragma unroll
             for (int i = 0; i < HELD; i++)
             {
@@ -697,8 +702,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 #pragma unroll
         for (int k = 0; k < 4; k++)
         {
-            r[k] = factors[0][quad_at<VEC>(lane, k)];
-            pull[k] = factors[1][quad_at<VEC>(lane, k)];
+            r[k] = factors[0][quad_at<VEC, LANES>(lane, k)];
+            pull[k] = factors[1][quad_at<VEC, LANES>(lane, k)];
         }
         fetch_wait<1>();   // gsum is here, the next tile may travel
         int64_t at = here.first;
@@ -711,7 +716,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
             s[i].values(v);
             widen_quad(gy[i], up);
             weight_sum[i] += quad_gradient(v, up, weight_of(i), r, pull, gx);
-            put_gradient<VEC, T>(a, gx, more_slot + i * COUNT, at, i < own ? here.left : 0);
+            put_gradient<VEC, LANES, T>(a, gx, more_slot + i * COUNT, at, i < own ? here.left : 0);
         }
         __syncwarp();
         if (!last) fetch_more(p);
@@ -722,8 +727,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 #pragma unroll
     for (int i = 0; i < HELD; i++)
     {
-        const W total = warp_sum(weight_sum[i]);
-        if (lane == 0 && i < own) partial[warp + i * WARPS] = total;
+        const W total = lanes_sum<LANES>(weight_sum[i]);
+        if (lane == 0 && i < own) partial[group + i * STEP] = total;
     }
 }
 
@@ -758,7 +763,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
                 gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + at, i0 + i < own ? p.left : 0);
             }
         };
-        tile_gradient_factors<VEC>(part, factors, C, a.eps, lane, warp, [&](auto& sums) {
+        tile_gradient_factors<VEC, 32>(part, factors, C, a.eps, lane, warp, [&](auto& sums) {
             for (int i0 = 0; i0 < own; i0 += HELD)
             {
                 load(i0);
@@ -802,7 +807,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
                     const W total = warp_sum(through);
                     if (lane == 0 && i0 + i < own) weight_sums[warp + (i0 + i) * WARPS] += total;   // the channel belongs to this warp alone
                 }
-                put_gradient<VEC, T>(a, gx, more + i, at, i0 + i < own ? p.left : 0);
+                put_gradient<VEC, 32, T>(a, gx, more + i, at, i0 + i < own ? p.left : 0);
             }
         }
     }
@@ -943,7 +948,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
                 gx[k] = r * (up[k] * g[k] - v[k] * pull);
                 weight_sum[i][k] += up[k] * (v[k] * r);
             }
-            put_gradient<VEC, T>(a, gx, &more, first + i * step, left_of(i, own));
+            put_gradient<VEC, 32, T>(a, gx, &more, first + i * step, left_of(i, own));
         }
         if (AHEAD)
         {

@@ -83,25 +83,27 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
         return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, true, 4, 8, 2>>(grid, 8, std::max(FEW, sums), stream, ROWS, a,
                                                                                        warps_per_row(a.tiles_per_row, 4, 8));
     }
-    if (a.channels <= 32) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2>>(grid, 8, FEW, stream, COLUMNS, a);
-    if constexpr (sizeof(T) == 8)
+    constexpr size_t MORE = gradient_slot_bytes<T, CODES>(8, 256);
+    if (a.channels <= 32) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 1, 2>>(grid, 8, FEW, stream, COLUMNS, a);
+    if constexpr (sizeof(T) == 8)   // eight quads of doubles do not fit the registers
     {
-        if (a.channels <= 64)
-            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(4, 512), stream, COLUMNS, a);
+        if (a.channels <= 64) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2, 2>>(grid, 8, FEW, stream, COLUMNS, a);
+        if (a.channels <= 128) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 4, 2>>(grid, 8, FEW, stream, COLUMNS, a);
     }
     else
     {
-        if (a.channels <= 64)
-            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2>>(grid, 8, gradient_slot_bytes<T, CODES>(8, 256), stream, COLUMNS, a);
-        if (a.channels <= 128)
-            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(8, 512), stream, COLUMNS, a);
+        if (a.channels <= 64) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 1, 2>>(grid, 8, MORE, stream, COLUMNS, a);
+        if (a.channels <= 128) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2, 2>>(grid, 8, MORE, stream, COLUMNS, a);
+        if (a.channels <= 256) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 4, 2>>(grid, 8, MORE, stream, COLUMNS, a);
+        if (a.channels <= 512)
+            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 4, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(8, 512), stream, COLUMNS, a);
     }
     return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
 }
 
 template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
-    const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner);
+    const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T) == 8);
     const int rc = backward_sums<T, VEC, CODES>(a, rows, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
     norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(

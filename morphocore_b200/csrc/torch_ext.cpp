@@ -78,6 +78,14 @@ void require_cuda(const torch::Tensor& t, const char* what)
     TORCH_CHECK(t.is_cuda(), "morphocore_b200 runs on CUDA devices only and has no CPU path: ", what, " is on ", t.device());
 }
 
+/// A new tensor beside `like`, straight from the allocator: the dispatcher's part of at::empty is 0.5 us of host time, up to
+/// five times an operator.
+torch::Tensor room(c10::IntArrayRef sizes, const torch::Tensor& like, torch::ScalarType dtype)
+{
+    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
+}
+torch::Tensor room_like(const torch::Tensor& like) { return room(like.sizes(), like, like.scalar_type()); }
+
 mc_desc make_desc(const torch::Tensor& input4d, const torch::Tensor& weight4d, int64_t op, int64_t merge)
 {
     mc_desc d{};
@@ -116,13 +124,6 @@ int storage_dtype_of(const torch::Tensor& t)
 }
 
 torch::ScalarType scale_type_of(torch::ScalarType t) { return t == torch::kDouble ? torch::kDouble : torch::kFloat; }
-
-/// A new tensor beside `like`, straight from the allocator: the dispatcher's part of at::empty is 0.5 us of host time, four times in the norm.
-torch::Tensor room(c10::IntArrayRef sizes, const torch::Tensor& like, torch::ScalarType dtype)
-{
-    return at::detail::empty_cuda(sizes, dtype, like.device(), std::nullopt);
-}
-torch::Tensor room_like(const torch::Tensor& like) { return room(like.sizes(), like, like.scalar_type()); }
 
 int64_t product(c10::IntArrayRef sizes) { return c10::multiply_integers(sizes); }
 
@@ -296,9 +297,9 @@ MorphoCall run_morpho_forward(const torch::Tensor& input, const torch::Tensor& w
     }
     const torch::Tensor& kernel_weight = call.sample_weight.defined() ? call.sample_weight : weight4d;
 
-    call.output = at::empty({input4d.size(0), weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d.options());
+    call.output = room({input4d.size(0), weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d, input4d.scalar_type());
     if (save_indices && (merge == MC_MERGE_MAX || merge == MC_MERGE_MIN))
-        call.indices = at::empty(call.output.sizes(), input4d.options().dtype(torch::kInt));
+        call.indices = room(call.output.sizes(), input4d, torch::kInt);
 
     const TraceRange trace("morphocore::morpho_forward");
     if (packed != nullptr && identity && d.dtype == MC_F32 && static_cast<int64_t>(d.H) * d.W > 1)
@@ -387,7 +388,7 @@ public:
         TORCH_CHECK(grad_output.scalar_type() == weight.scalar_type(), "grad_output must have the same dtype as input");
 
         const c10::cuda::CUDAGuard device_guard(weight.device());
-        torch::Tensor grad_input = torch::empty(input_sizes, weight.options());
+        torch::Tensor grad_input = room(input_sizes, weight, weight.scalar_type());
         mc_desc d = make_desc(grad_input, weight, ctx->saved_data["op"].toInt(), ctx->saved_data["merge"].toInt());
         d.pad_kind = static_cast<int32_t>(ctx->saved_data["pad_kind"].toInt());
         d.fill = ctx->saved_data["fill"].toDouble();
@@ -396,11 +397,11 @@ public:
         const torch::Tensor& kernel_weight = sample_weight.defined() ? sample_weight : weight;
         if (sample_weight.defined()) d.weight_batch_stride = weight.numel();
 
-        torch::Tensor grad_weight = torch::empty_like(weight);
+        torch::Tensor grad_weight = room_like(weight);
         const bool have_idx = indices.defined() && indices.numel() > 0;
         const size_t ws_bytes = mc_morpho_backward_workspace_bytes(&d, have_idx);
         torch::Tensor workspace;
-        if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, weight.options().dtype(torch::kByte));
+        if (ws_bytes > 0) workspace = room({static_cast<int64_t>(ws_bytes)}, weight, torch::kByte);
         const TraceRange trace("morphocore::morpho_backward");
         if (!identity_backward_8bit(d, saved[4], saved[5], kernel_weight, grad_output, grad_input, grad_weight))
         {
@@ -447,8 +448,8 @@ MorphoPairCall run_morpho_pair_forward(const torch::Tensor& input, const torch::
     mc_desc d = make_desc(input4d, weight4d, MC_OP_DILATION, merge);
     d.pad_kind = padding == PAD_REPLICATE ? MC_PAD_REPLICATE : MC_PAD_FILL;
     d.fill = fill_value(MC_OP_DILATION, padding, padding_value, d.dtype == MC_F32);
-    call.out_dilation = at::empty({input4d.size(0), weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d.options());
-    call.out_erosion = at::empty_like(call.out_dilation);
+    call.out_dilation = room({input4d.size(0), weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d, input4d.scalar_type());
+    call.out_erosion = room_like(call.out_dilation);
     void* const dilation_out = call.out_dilation.data_ptr();
     void* const erosion_out = call.out_erosion.data_ptr();
     const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
@@ -524,12 +525,12 @@ public:
             d.flags = (op == MC_OP_EROSION ? MC_FLAG_FLIPPED_WEIGHT : 0) | (grad_input.defined() ? MC_FLAG_ACCUMULATE : 0);
             if (!grad_input.defined())
             {
-                grad_input = at::empty_like(input);
-                grad_weight = at::empty_like(weight);
+                grad_input = room_like(input);
+                grad_weight = room_like(weight);
             }
             const size_t ws_bytes = mc_morpho_backward_workspace_bytes(&d, 0);
             torch::Tensor workspace;
-            if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, input.options().dtype(torch::kByte));
+            if (ws_bytes > 0) workspace = room({static_cast<int64_t>(ws_bytes)}, input, torch::kByte);
             const TraceRange trace("morphocore::morpho_backward");
             check_status(mc_morpho_backward(&d, input.data_ptr(), weight.data_ptr(), nullptr, grad_output.data_ptr(), grad_input.data_ptr(),
                                             grad_weight.data_ptr(), workspace.defined() ? workspace.data_ptr() : nullptr, ws_bytes, stream));
@@ -562,7 +563,7 @@ struct SmorphCall
 /// w~ of the pairs (mc_smorph_reparametrise).
 torch::Tensor reparametrised(const mc_desc& d, const torch::Tensor& weight4d, const torch::Tensor& alphas, cudaStream_t stream)
 {
-    torch::Tensor out = at::empty_like(weight4d);
+    torch::Tensor out = room_like(weight4d);
     check_status(mc_smorph_reparametrise(&d, weight4d.data_ptr(), alphas.data_ptr(), out.data_ptr(), stream));
     return out;
 }
@@ -599,7 +600,7 @@ SmorphCall run_smorph_forward(const torch::Tensor& input, const torch::Tensor& w
     const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
     const TraceRange trace("morphocore::smorph_forward");
     if (reparametrise) call.weight4d = reparametrised(d, call.weight4d, call.alphas, stream);
-    call.output = at::empty({input4d.size(0), call.weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d.options());
+    call.output = room({input4d.size(0), call.weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d, input4d.scalar_type());
     check_status(mc_smorph_forward(&d, input4d.data_ptr(), call.weight4d.data_ptr(), call.alphas.data_ptr(), call.output.data_ptr(), stream));
     return call;
 }
@@ -622,7 +623,7 @@ torch::Tensor through_reparametrisation(const mc_desc& d, const torch::Tensor& w
         return t * (straight * grad + mirrored * grad.flip({2, 3}));
     }
     const torch::Tensor raw = weight.defined() ? weight.contiguous() : w_tilde;
-    torch::Tensor out = at::empty_like(grad);
+    torch::Tensor out = room_like(grad);
     check_status(mc_smorph_reparametrise_backward(&d, raw.data_ptr(), alphas.data_ptr(), grad.data_ptr(), out.data_ptr(), grad_alpha_pairs.data_ptr(),
                                                   stream));
     return out;
@@ -685,16 +686,16 @@ public:
         const mc_desc d = make_desc(input, weight, MC_OP_DILATION, merge);
         if (saved[6].defined() && (merge == MC_MERGE_MAX || merge == MC_MERGE_MIN))
         {
-            output = at::empty(output_sizes, weight.options());
+            output = room(output_sizes, weight, weight.scalar_type());
             check_status(mc_smorph_forward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), output.data_ptr(),
                                            at::cuda::getCurrentCUDAStream().stream()));
         }
-        torch::Tensor grad_input = torch::empty_like(input);
-        torch::Tensor grad_weight = torch::empty_like(weight);
-        torch::Tensor grad_alpha_pairs = torch::empty_like(alphas);
+        torch::Tensor grad_input = room_like(input);
+        torch::Tensor grad_weight = room_like(weight);
+        torch::Tensor grad_alpha_pairs = room_like(alphas);
         const size_t ws_bytes = mc_smorph_backward_workspace_bytes(&d);
         torch::Tensor workspace;
-        if (ws_bytes > 0) workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, input.options().dtype(torch::kByte));
+        if (ws_bytes > 0) workspace = room({static_cast<int64_t>(ws_bytes)}, input, torch::kByte);
 
         const TraceRange trace("morphocore::smorph_backward");
         const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
@@ -748,7 +749,7 @@ SmorphScmCall run_smorph_scm_forward(const torch::Tensor& input, const torch::Te
     const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
     const TraceRange trace("morphocore::smorph_scm_forward");
     if (reparametrise) call.weight4d = reparametrised(d, call.weight4d, call.alphas, stream);
-    call.output = at::empty({input4d.size(0), call.weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d.options());
+    call.output = room({input4d.size(0), call.weight4d.size(0), input4d.size(2), input4d.size(3)}, input4d, input4d.scalar_type());
     check_status(mc_smorph_scm_forward(&d, input4d.data_ptr(), call.weight4d.data_ptr(), call.alphas.data_ptr(), call.betas.data_ptr(),
                                        call.output.data_ptr(), stream));
     return call;
@@ -803,16 +804,16 @@ public:
         const mc_desc d = make_desc(input, weight, MC_OP_DILATION, MC_MERGE_SMOOTH);
         if (saved[7].defined())
         {
-            output = at::empty(output_sizes, weight.options());
+            output = room(output_sizes, weight, weight.scalar_type());
             check_status(mc_smorph_scm_forward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), beta.data_ptr(), output.data_ptr(),
                                                at::cuda::getCurrentCUDAStream().stream()));
         }
-        torch::Tensor grad_input = torch::empty_like(input);
-        torch::Tensor grad_weight = torch::empty_like(weight);
-        torch::Tensor grad_alpha_pairs = torch::empty_like(alphas);
-        torch::Tensor grad_beta = torch::empty_like(beta);
+        torch::Tensor grad_input = room_like(input);
+        torch::Tensor grad_weight = room_like(weight);
+        torch::Tensor grad_alpha_pairs = room_like(alphas);
+        torch::Tensor grad_beta = room_like(beta);
         const size_t ws_bytes = mc_smorph_scm_backward_workspace_bytes(&d);
-        torch::Tensor workspace = torch::empty({static_cast<int64_t>(ws_bytes)}, input.options().dtype(torch::kByte));
+        torch::Tensor workspace = room({static_cast<int64_t>(ws_bytes)}, input, torch::kByte);
         const TraceRange trace("morphocore::smorph_scm_backward");
         const cudaStream_t stream = at::cuda::getCurrentCUDAStream().stream();
         check_status(mc_smorph_scm_backward(&d, input.data_ptr(), weight.data_ptr(), alphas.data_ptr(), beta.data_ptr(), output.data_ptr(),
