@@ -47,6 +47,7 @@ template <typename Args> void set_sizes(Args& a, const mc_norm_desc& d)
     a.tiles_per_row = code_blocks(d.inner == 1 ? d.channels : d.inner);
     a.tiles = d.outer * a.tiles_per_row;
     a.eps = d.eps;
+    a.per_channel = 1.0 / static_cast<double>(d.channels);
 }
 
 int refuse(const char* why)
@@ -55,7 +56,7 @@ int refuse(const char* why)
     return MC_ERR_INVALID_ARGUMENT;
 }
 
-size_t wide_bytes(const mc_norm_desc& d) { return d.dtype == MC_F64 ? 8 : 4; }
+int element_bytes(const mc_norm_desc& d) { return d.dtype == MC_F64 ? 8 : d.dtype == MC_F32 ? 4 : 2; }
 
 }  // namespace
 
@@ -86,7 +87,8 @@ int mc_rms_norm_forward(const mc_norm_desc* desc, const void* x, const void* res
 size_t mc_rms_norm_backward_workspace_bytes(const mc_norm_desc* desc, int have_gweight)
 {
     if (!have_gweight || checked_norm(desc) != MC_OK || desc->outer * desc->inner == 0) return 0;
-    return wide_bytes(*desc) * static_cast<size_t>(norm_backward_grid(desc->outer, desc->channels, desc->inner, desc->dtype == MC_F64)) * static_cast<size_t>(desc->channels);
+    const bool wide = desc->dtype == MC_F64;
+    return (wide ? 8 : 4) * static_cast<size_t>(norm_backward_grid(desc->outer, desc->channels, desc->inner, wide)) * static_cast<size_t>(desc->channels);
 }
 
 int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t* sum_codes, const void* sum_scales, const void* weight, const void* gy,
@@ -98,8 +100,7 @@ int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t
     if (desc->outer * desc->inner == 0)
     {
         if (gweight == nullptr) return MC_OK;
-        const size_t element = desc->dtype == MC_F64 ? 8 : desc->dtype == MC_F32 ? 4 : 2;
-        const cudaError_t err = cudaMemsetAsync(gweight, 0, element * static_cast<size_t>(desc->channels), static_cast<cudaStream_t>(stream));
+        const cudaError_t err = cudaMemsetAsync(gweight, 0, static_cast<size_t>(element_bytes(*desc)) * static_cast<size_t>(desc->channels), static_cast<cudaStream_t>(stream));
         if (err == cudaSuccess) return MC_OK;
         set_last_error("cudaMemsetAsync: %s", cudaGetErrorString(err));
         return MC_ERR_CUDA;

@@ -27,7 +27,7 @@ struct NormArgs
     int8_t *y_codes, *sum_codes;
     int64_t outer, channels, inner;
     int64_t tiles_per_row, tiles;   // blocks of 128 pixels in an image and in all (columns), of 128 channels in a row (rows)
-    double eps;
+    double eps, per_channel;        // per_channel: 1 / channels
 };
 
 struct NormGradArgs
@@ -38,7 +38,7 @@ struct NormGradArgs
     void* partial;                  // [grid, channels], Wide<T>
     int64_t outer, channels, inner;
     int64_t tiles_per_row, tiles;
-    double eps;
+    double eps, per_channel;
 };
 
 /// What the forward kernels add squares up in.
@@ -54,6 +54,7 @@ template <typename T> struct Factor
 {
     Wide<T> r;
     __device__ __forceinline__ void set(double v) { r = static_cast<Wide<T>>(v); }
+    __device__ __forceinline__ Factor of_lane(int i) const { return {__shfl_sync(0xffffffffu, r, i)}; }
 };
 template <> struct Factor<float>
 {
@@ -63,6 +64,7 @@ template <> struct Factor<float>
         r = static_cast<float>(v);
         low = static_cast<float>(v - static_cast<double>(r));
     }
+    __device__ __forceinline__ Factor of_lane(int i) const { return {__shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, low, i)}; }
 };
 
 template <typename T> __device__ __forceinline__ void times(const Wide<T> (&s)[4], const Factor<T>& r0, const Factor<T>& r1, const Factor<T>& r2,
@@ -96,6 +98,9 @@ __device__ __forceinline__ bool ordinary_weight(float g) { return fabsf(g) < 0x1
 __device__ __forceinline__ bool ordinary_weight(double) { return true; }
 
 __device__ __forceinline__ bool ordinary(double r) { return r > 0x1p-60 && r < 0x1p60; }
+
+/// r from the sum of the squares.
+__device__ __forceinline__ double norm_factor(double squares, double per_channel, double eps) { return rsqrt(squares * per_channel + eps); }
 
 /// Sums in float are taken once more in double where they left its range: squares near its largest value, or, for an eps that does not
 /// cover them, near its smallest; infinities and NaN.
@@ -131,7 +136,7 @@ template <typename T> __device__ __forceinline__ Quad<T> add_quads(const Quad<T>
     return narrow_quad<T>(u);
 }
 
-/// Sums of squares of N quads, one a lane's element or one for all four, added to `sums`.
+/// Sums of squares of N quads, one, two or four for a lane's four elements, added to `sums`.
 template <int N, int SUMS, typename T, typename S> __device__ __forceinline__ void add_squares(const Quad<T> (&s)[N], S (&sums)[SUMS])
 {
 #pragma unroll
@@ -144,10 +149,10 @@ template <int N, int SUMS, typename T, typename S> __device__ __forceinline__ vo
     }
 }
 
-/// Codes and scales of N blocks, of which the first of lane and the others `step` elements and `block_step` blocks apart; `count` exist.
-/// `scales` is where the scale of the first goes.
-template <bool VEC, int N, typename T>
-__device__ __forceinline__ void put_codes(int8_t* codes, void* scales, int64_t step, int64_t block_step, const Quad<T> (&q)[N], int count, int lane, const int (&left)[N])
+/// Codes and scales of N blocks: block i lies `offset(i)` elements and i `block_step` blocks behind the first, whose codes and scale go to `codes`
+/// and `scales`; `count` exist.
+template <bool VEC, int N, typename T, typename Offset>
+__device__ __forceinline__ void put_codes(int8_t* codes, void* scales, Offset offset, int64_t block_step, const Quad<T> (&q)[N], int count, int lane, const int (&left)[N])
 {
     Wide<T> v[N][4];
     uint32_t c[N];
@@ -155,7 +160,7 @@ __device__ __forceinline__ void put_codes(int8_t* codes, void* scales, int64_t s
     for (int i = 0; i < N; i++) widen_quad(q[i], v[i]);
     const Wide<T> scale = encode_blocks(v, c, lane);
 #pragma unroll
-    for (int i = 0; i < N; i++) store_codes<VEC>(codes + i * step, c[i], left[i]);
+    for (int i = 0; i < N; i++) store_codes<VEC>(codes + offset(i), c[i], left[i]);
     if (lane < count) static_cast<Wide<T>*>(scales)[lane * block_step] = scale;
 }
 
@@ -233,6 +238,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
     const int own = (C - warp + WARPS - 1) / WARPS;   // channels of this warp
     const bool held = C <= HELD * WARPS;
     const int64_t step = WARPS * a.inner, block_step = WARPS * a.tiles_per_row;
+    const auto offset = [&](int i) { return i * step; };
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
         const int64_t image = tile / a.tiles_per_row, piece = tile - image * a.tiles_per_row;
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
                     if (at >= own) break;
                     const Quad<T> q[GROUP] = {s[g0], s[g0 + 1], s[g0 + 2], s[g0 + 3]};
                     const int lefts[GROUP] = {left, at + 1 < own ? left : 0, at + 2 < own ? left : 0, at + 3 < own ? left : 0};
-                    put_codes<VEC>(a.sum_codes + first + at * step, static_cast<W*>(a.sum_scales) + first_block + at * block_step, step, block_step, q,
+                    put_codes<VEC>(a.sum_codes + first + at * step, static_cast<W*>(a.sum_scales) + first_block + at * block_step, offset, block_step, q,
                                    own - at, lane, lefts);
                 }
         }
@@ -283,7 +289,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
             double total = 0.0;
 #pragma unroll
             for (int w = 0; w < WARPS; w++) total += part[w][threadIdx.x];
-            factor[threadIdx.x] = 1.0 / sqrt(total / static_cast<double>(C) + a.eps);
+            factor[threadIdx.x] = norm_factor(total, a.per_channel, a.eps);
             return total;
         };
         __syncthreads();
@@ -354,123 +360,182 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
                     for (int i = 0; i < GROUP; i++, p += step) store_quad<VEC>(p, y[i], lefts[i]);
                 }
                 if (a.y_codes != nullptr)
-                    put_codes<VEC>(a.y_codes + first + at * step, static_cast<W*>(a.y_scales) + first_block + at * block_step, step, block_step, y, own - at, lane,
+                    put_codes<VEC>(a.y_codes + first + at * step, static_cast<W*>(a.y_scales) + first_block + at * block_step, offset, block_step, y, own - at, lane,
                                    lefts);
             }
         }
     }
 }
 
-/// Sum over the `per_row` warps of a group, which share a row; every warp of the thread block calls it. Within a warp in the type of v, the warps'
-/// sums in double.
-template <int WARPS, typename V> __device__ __forceinline__ double group_sum(V v, double (&part)[WARPS], int per_row)
+/// Sums over the warp of R values (1, 2 or 4): lane l returns that of value l % R. A lane gives away the values that others will hold.
+template <int R, typename V> __device__ __forceinline__ V spread_sums(const V (&v)[R], int lane)
 {
-    const double own = static_cast<double>(warp_sum(v));
-    if (per_row == 1) return own;
-    const int warp = threadIdx.x >> 5, leader = warp / per_row * per_row;
-    __syncthreads();   // the sums of the row before have been read
-    if ((threadIdx.x & 31) == 0) part[warp] = own;
-    __syncthreads();
-    double total = 0.0;
-    for (int w = 0; w < per_row; w++) total += part[leader + w];
-    return total;
+    static_assert(R == 1 || R == 2 || R == 4, "a power of two");
+    const auto halve = [&](V even, V odd, int d) {
+        const bool upper = (lane & d) != 0;
+        return (upper ? odd : even) + __shfl_xor_sync(0xffffffffu, upper ? even : odd, d);
+    };
+    V sum;
+    if constexpr (R == 1) sum = v[0];
+    else if constexpr (R == 2) sum = halve(v[0], v[1], 1);
+    else sum = halve(halve(v[0], v[1], 1), halve(v[2], v[3], 1), 2);
+#pragma unroll
+    for (int d = R; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
 }
 
-/// Forward, rows of channels: `per_row` warps (a power of two) take a row, warp w of them the blocks w, w + per_row, ... of 128
-/// channels, at most HELD of them.
-template <typename T, bool VEC, int HELD, int WARPS, int CTAS>
-__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int per_row)
+/// Adds up K numbers of each of the 2^shift warps that share a row; every lane gets the sums. The warps of a row meet at a barrier of their own:
+/// `part` is written in turns, so that one is enough.
+template <int K, int WARPS> __device__ __forceinline__ void share_sums(double (&v)[K], double (&part)[2][WARPS][K], int& turn, int shift)
 {
-    static_assert(HELD % GROUP == 0, "whole groups");
-    using W = Wide<T>;
-    __shared__ double part[WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % per_row, groups = WARPS / per_row;
-    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row), step = per_row * CODE_BLOCK;
-    const int c0 = sub * CODE_BLOCK + lane_at<VEC>(lane);   // the lane's first channel
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < a.outer; row0 += static_cast<int64_t>(gridDim.x) * groups)
-    {
-        const int64_t row = row0 + warp / per_row, first = row * C + c0;
-        const int64_t first_block = row * blocks + sub;
-        const int own = row < a.outer ? (blocks - sub + per_row - 1) / per_row : 0;   // a warp without a row still takes part in the sums
-        // What lies from the lane's element of block i to the end of the block.
-        const auto left_of = [&](int i) { return i < own ? min(CODE_BLOCK - lane_at<VEC>(lane), C - c0 - i * step) : 0; };
-        Quad<T> s[HELD];
-        const auto load = [&](const void* from, int64_t at, Quad<T> (&q)[HELD]) {
+    if (shift == 0) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp >> shift, per_row = 1 << shift;
+    if (lane == 0)
 #pragma unroll
-            for (int i = 0; i < HELD; i++) q[i] = load_quad<VEC>(static_cast<const T*>(from) + at + i * step, left_of(i));
+        for (int k = 0; k < K; k++) part[turn][warp][k] = v[k];
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "r"(32 << shift) : "memory");
+#pragma unroll
+    for (int k = 0; k < K; k++) v[k] = part[turn][(group << shift) + (lane & (per_row - 1))][k];
+    turn ^= 1;
+    for (int d = per_row >> 1; d > 0; d >>= 1)
+#pragma unroll
+        for (int k = 0; k < K; k++) v[k] += __shfl_xor_sync(0xffffffffu, v[k], d);
+}
+
+/// How a warp of the kernels for rows of channels holds ROWS neighbouring rows of BLOCKS blocks of 128 channels each; 2^shift warps share a row, warp
+/// `sub` of them has the blocks sub, sub + 2^shift, ... More than one row is for rows of exactly BLOCKS blocks that no warps share. Without that a row
+/// of few channels leaves most of what a warp is unrolled for empty: (65536, 64) in float took 45 us, ROWS_FEW so.
+template <bool VEC, int ROWS, int BLOCKS> struct RowTile
+{
+    int C, c0, own, step, at;   // channels; the lane's first; blocks of this warp; channels from one to the next; the lane's place in a block
+
+    __device__ __forceinline__ RowTile(int64_t channels, int64_t blocks, int shift, int lane, int warp)
+        : C(static_cast<int>(channels)), step(CODE_BLOCK << shift), at(lane_at<VEC>(lane))
+    {
+        const int sub = warp & ((1 << shift) - 1);
+        c0 = sub * CODE_BLOCK + at;
+        own = (static_cast<int>(blocks) - sub + (1 << shift) - 1) >> shift;
+    }
+    /// Channels from the lane's of block j to the end of the block.
+    __device__ __forceinline__ int left_in(int j) const { return j < own ? min(CODE_BLOCK - at, C - c0 - j * step) : 0; }
+    /// The same for quad q, of `rows` rows that exist; where it lies; and how many blocks there are.
+    __device__ __forceinline__ int left(int q, int rows) const { return q / BLOCKS < rows ? left_in(q % BLOCKS) : 0; }
+    __device__ __forceinline__ int offset(int q) const { return q / BLOCKS * C + q % BLOCKS * step; }
+    __device__ __forceinline__ int count(int rows) const { return ROWS == 1 ? own : rows * BLOCKS; }
+};
+
+/// Forward, rows of channels.
+template <typename T, bool VEC, int ROWS, int BLOCKS, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int shift)
+{
+    constexpr int N = ROWS * BLOCKS;
+    static_assert(N % GROUP == 0, "whole groups");
+    using W = Wide<T>;
+    __shared__ double part[2][WARPS][1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = WARPS >> shift;
+    const RowTile<VEC, ROWS, BLOCKS> t(a.channels, a.tiles_per_row, shift, lane, warp);
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * ROWS;
+    int turn = 0;
+    for (int64_t row = (static_cast<int64_t>(blockIdx.x) * groups + (warp >> shift)) * ROWS; row < a.outer; row += stride)
+    {
+        const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), a.outer - row)), count = t.count(rows);
+        const int64_t first = row * t.C + t.c0, first_block = row * a.tiles_per_row + (t.c0 - t.at) / CODE_BLOCK;
+        Quad<T> s[N];
+        const auto load = [&](const void* from, Quad<T> (&q)[N]) {
+#pragma unroll
+            for (int i = 0; i < N; i++) q[i] = load_quad<VEC>(static_cast<const T*>(from) + first + t.offset(i), t.left(i, rows));
         };
-        load(a.x, first, s);
+        load(a.x, s);
         if (a.residual != nullptr)
         {
-            Quad<T> more[HELD];
-            load(a.residual, first, more);
+            Quad<T> more[N];
+            load(a.residual, more);
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int i = 0; i < N; i++)
             {
                 s[i] = add_quads(s[i], more[i]);
-                store_quad<VEC>(static_cast<T*>(a.sum) + first + i * step, s[i], left_of(i));
+                store_quad<VEC>(static_cast<T*>(a.sum) + first + t.offset(i), s[i], t.left(i, rows));
             }
         }
-        Sum<T> sums[1] = {};
-        add_squares(s, sums);
+        const auto add_up = [&](auto zero) {   // the squares of row lane % ROWS
+            decltype(zero) sums[ROWS][2] = {};
+#pragma unroll
+            for (int i = 0; i < N; i++)
+            {
+                const Quad<T> one[1] = {s[i]};
+                add_squares(one, sums[i / BLOCKS]);
+            }
+            decltype(zero) own[ROWS];
+#pragma unroll
+            for (int i = 0; i < ROWS; i++) own[i] = sums[i][0] + sums[i][1];
+            double total[1] = {static_cast<double>(spread_sums(own, lane))};
+            share_sums(total, part, turn, shift);
+            return total[0];
+        };
         const auto put = [&](int8_t* codes, void* scales, const Quad<T> (&q)[GROUP], int g0) {
-            const int lefts[GROUP] = {left_of(g0), left_of(g0 + 1), left_of(g0 + 2), left_of(g0 + 3)};
-            put_codes<VEC>(codes + first + g0 * step, static_cast<W*>(scales) + first_block + g0 * per_row, step, per_row, q, own - g0, lane, lefts);
+            const int lefts[GROUP] = {t.left(g0, rows), t.left(g0 + 1, rows), t.left(g0 + 2, rows), t.left(g0 + 3, rows)};
+            put_codes<VEC>(codes + first, static_cast<W*>(scales) + first_block + (static_cast<int64_t>(g0) << shift), [&](int i) { return t.offset(g0 + i); },
+                           int64_t(1) << shift, q, count - g0, lane, lefts);
         };
         if (a.sum_codes != nullptr)
 #pragma unroll
-            for (int g0 = 0; g0 < HELD; g0 += GROUP)
+            for (int g0 = 0; g0 < N; g0 += GROUP)
             {
-                if (g0 >= own) break;
+                if (g0 >= count) break;
                 const Quad<T> q[GROUP] = {s[g0], s[g0 + 1], s[g0 + 2], s[g0 + 3]};
                 put(a.sum_codes, a.sum_scales, q, g0);
             }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
-        double total = group_sum<WARPS>(sums[0], part, per_row);
-        if (sizeof(Sum<T>) == 4)
+        double total = add_up(Sum<T>(0));
+        // Squares that left the range of float, or would where eps does not cover them: in double. The warps that share a row agree.
+        if (sizeof(Sum<T>) == 4 && __any_sync(0xffffffffu, out_of_range(total, 0.0, a.eps)))
         {
-            // Squares that left the range of float, or would where eps does not cover them: in double. The warps of a row agree; where
-            // rows are shared the thread block decides as one, because its barriers are in common.
-            bool again = out_of_range(total, 0.0, a.eps);
-            if (per_row > 1) again = __syncthreads_or(again);
-            if (again)
-            {
-                double exact[1] = {};
-                add_squares(s, exact);
-                total = group_sum<WARPS>(exact[0], part, per_row);
-            }
+            rarely();
+            total = add_up(0.0);
         }
-        const double factor = 1.0 / sqrt(total / static_cast<double>(C) + a.eps);
-        Factor<T> r;
-        r.set(factor);
+        const double factor = norm_factor(total, a.per_channel, a.eps);
+        const bool all_ordinary = __all_sync(0xffffffffu, ordinary(factor));
+        Factor<T> mine, r[ROWS];
+        mine.set(factor);
 #pragma unroll
-        for (int g0 = 0; g0 < HELD; g0 += GROUP)
+        for (int i = 0; i < ROWS; i++) r[i] = ROWS == 1 ? mine : mine.of_lane(i);
+        W g[4] = {1, 1, 1, 1};
+        bool usual = all_ordinary;
+#pragma unroll
+        for (int g0 = 0; g0 < N; g0 += GROUP)
         {
-            if (g0 >= own) break;
+            if (g0 >= count) break;
             Quad<T> y[GROUP];
 #pragma unroll
             for (int i = 0; i < GROUP; i++)
             {
-                W v[4], g[4] = {1, 1, 1, 1}, result[4];
-                widen_quad(s[g0 + i], v);
-                if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + c0 + (g0 + i) * step, left_of(g0 + i)), g);
-                if (ordinary(factor) && ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]))
-                    times(v, r, r, r, r, g, result);
-                else
+                const int q = g0 + i;
+                W v[4], result[4];
+                widen_quad(s[q], v);
+                if (a.weight != nullptr && (BLOCKS > 1 || q == 0))
+                {
+                    widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + q % BLOCKS * t.step, t.left_in(q % BLOCKS)), g);
+                    usual = all_ordinary && __all_sync(0xffffffffu, ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]));
+                }
+                const Factor<T>& f = r[q / BLOCKS];
+                if (usual) times(v, f, f, f, f, g, result);
+                else   // the whole warp
                 {
                     rarely();
+                    const double exact = __shfl_sync(0xffffffffu, factor, q / BLOCKS);
 #pragma unroll
-                    for (int k = 0; k < 4; k++) result[k] = static_cast<W>(static_cast<double>(v[k]) * factor * static_cast<double>(g[k]));
+                    for (int k = 0; k < 4; k++) result[k] = static_cast<W>(static_cast<double>(v[k]) * exact * static_cast<double>(g[k]));
                 }
                 y[i] = narrow_quad<T>(result);
-                if (a.y != nullptr) store_quad<VEC>(static_cast<T*>(a.y) + first + (g0 + i) * step, y[i], left_of(g0 + i));
+                if (a.y != nullptr) store_quad<VEC>(static_cast<T*>(a.y) + first + t.offset(q), y[i], t.left(q, rows));
             }
             if (a.y_codes != nullptr) put(a.y_codes, a.y_scales, y, g0);
         }
     }
 }
 
-/// What the backward kernels hold of a block of s: the elements, or four codes a lane and their scale.
+/// What the backward kernels hold of a block of s: the elements, or four codes a lane and their scale, which in float and double are fewer registers than
+/// the elements; in half precision they are as many, and the elements are made once.
 template <typename T, bool CODES> struct HeldSum
 {
     Quad<T> q;
@@ -489,37 +554,50 @@ template <typename T, bool CODES> struct HeldSum
 };
 template <typename T> struct HeldSum<T, true>
 {
-    uint32_t codes;
-    Wide<T> scale;
+    static constexpr bool DECODED = sizeof(T) == 2;
+    struct Codes
+    {
+        uint32_t codes;
+        Wide<T> scale;
+    };
+    typename std::conditional<DECODED, Quad<T>, Codes>::type held;
+    using Slot = uint32_t;
     template <bool VEC> __device__ __forceinline__ void load(const NormGradArgs& a, int64_t at, int64_t block, int left, bool exists)
     {
-        codes = load_codes<VEC>(a.sum_codes + at, left);
-        scale = exists ? __ldg(static_cast<const Wide<T>*>(a.sum_scales) + block) : Wide<T>(0);
+        take(load_codes<VEC>(a.sum_codes + at, left), exists ? __ldg(static_cast<const Wide<T>*>(a.sum_scales) + block) : Wide<T>(0));
     }
-    using Slot = uint32_t;
     template <bool VEC, int LANES = 32> static __device__ __forceinline__ void fetch(const NormGradArgs& a, Slot* slot, int64_t at, int left)
     {
         fetch_codes<VEC, LANES>(slot, a.sum_codes, at, left);
     }
-    __device__ __forceinline__ void take(const Slot& slot, Wide<T> s)
+    __device__ __forceinline__ void take(uint32_t codes, Wide<T> scale)
     {
-        codes = slot;
-        scale = s;
+        if constexpr (DECODED)
+        {
+            Wide<T> v[4];
+            decode_quad(codes, scale, v);
+            held = narrow_quad<T>(v);
+        }
+        else held = {codes, scale};
     }
-    __device__ __forceinline__ void forget_values() { asm("" : "+r"(codes)); }
+    __device__ __forceinline__ void forget_values()
+    {
+        if constexpr (DECODED) forget_widened(held);
+        else asm("" : "+r"(held.codes));
+    }
     __device__ __forceinline__ void values(Wide<T> (&v)[4]) const
     {
-        decode_quad(codes, scale, v);
-        if constexpr (sizeof(T) == 2) widen_quad(narrow_quad<T>(v), v);
+        if constexpr (DECODED) widen_quad(held, v);
+        else decode_quad(held.codes, held.scale, v);
     }
 };
 
 /// The two numbers that a pixel's gradients need from its sums over the channels.
-template <typename W> __device__ __forceinline__ void gradient_factors(double squares, double products, double channels, double eps, W& r, W& pull)
+template <typename W> __device__ __forceinline__ void gradient_factors(double squares, double products, double per_channel, double eps, W& r, W& pull)
 {
-    const double factor = 1.0 / sqrt(squares / channels + eps);
+    const double factor = norm_factor(squares, per_channel, eps);
     r = static_cast<W>(factor);
-    pull = static_cast<W>(factor * factor * (products / channels));
+    pull = static_cast<W>(factor * factor * (products * per_channel));
 }
 
 /// gx of a lane's quad, `more` pointing to the gradient that comes past the norm.
@@ -539,7 +617,7 @@ template <bool VEC, int LANES, typename T> __device__ __forceinline__ void put_g
 /// products of the warp's channels up in the type that it is given, and again in double where float's range was left: squares and products in
 /// turn then, because the room is that of both in float. Ends with a barrier.
 template <bool VEC, int LANES, typename W, int GROUPS, int PIXELS, typename AddUp>
-__device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXELS], W (&factors)[2][PIXELS], int C, double eps, int lane, int group, AddUp add_up)
+__device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXELS], W (&factors)[2][PIXELS], double per_channel, double eps, int lane, int group, AddUp add_up)
 {
     W sums[2][4] = {};
     add_up(sums);
@@ -559,7 +637,7 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
             total[0] += static_cast<double>(part[0][g][threadIdx.x]);
             total[1] += static_cast<double>(part[1][g][threadIdx.x]);
         }
-        gradient_factors(total[0], total[1], static_cast<double>(C), eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
     }
     if constexpr (sizeof(W) == 8) __syncthreads();
     else if (__syncthreads_or(threadIdx.x < PIXELS && out_of_range(total[0], total[1], eps)))
@@ -580,7 +658,7 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
             }
             __syncthreads();
         }
-        if (threadIdx.x < PIXELS) gradient_factors(total[0], total[1], static_cast<double>(C), eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        if (threadIdx.x < PIXELS) gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
         __syncthreads();
     }
 }
@@ -688,7 +766,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
             fetch(p);
         }
         fetch_commit();
-        tile_gradient_factors<VEC, LANES>(part, factors, C, a.eps, lane, group, [&](auto& sums) {
+        tile_gradient_factors<VEC, LANES>(part, factors, a.per_channel, a.eps, lane, group, [&](auto& sums) {
 #pragma unroll
             for (int i = 0; i < HELD; i++)
             {
@@ -763,7 +841,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
                 gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + at, i0 + i < own ? p.left : 0);
             }
         };
-        tile_gradient_factors<VEC, 32>(part, factors, C, a.eps, lane, warp, [&](auto& sums) {
+        tile_gradient_factors<VEC, 32>(part, factors, a.per_channel, a.eps, lane, warp, [&](auto& sums) {
             for (int i0 = 0; i0 < own; i0 += HELD)
             {
                 load(i0);
@@ -818,45 +896,50 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
         if (lane == 0) partial[c] = weight_sums[c];
 }
 
-/// Backward, rows of channels; the next row of a warp is fetched while this one is computed (AHEAD: where the slots fit shared memory). gweight's
+/// Backward, rows of channels; what a warp takes next is fetched while this is computed (AHEAD: where the slots fit shared memory). gweight's
 /// sums stay in the lanes that have the channels; the groups of a thread block add theirs up in shared memory, one after the other, at the end.
-template <typename T, bool VEC, bool CODES, bool AHEAD, int HELD, int WARPS, int CTAS>
-__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kernel(const NormGradArgs a, int per_row)
+template <typename T, bool VEC, bool CODES, bool AHEAD, int ROWS, int BLOCKS, int WARPS, int CTAS>
+__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kernel(const NormGradArgs a, int shift)
 {
     using W = Wide<T>;
     using Held = HeldSum<T, CODES>;
-    constexpr int COUNT = WARPS * 32;
-    __shared__ double part[WARPS];
+    constexpr int COUNT = WARPS * 32, N = ROWS * BLOCKS;
+    __shared__ double part[2][WARPS][2];
     extern __shared__ __align__(16) unsigned char slots[];
-    Quad<T>* const gy_slot = reinterpret_cast<Quad<T>*>(slots) + threadIdx.x;   // [HELD][threads] each
-    Quad<T>* const more_slot = gy_slot + HELD * COUNT;
-    typename Held::Slot* const sum_slot = reinterpret_cast<typename Held::Slot*>(slots + 2 * HELD * COUNT * sizeof(Quad<T>)) + threadIdx.x;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % per_row, groups = WARPS / per_row;
-    const int C = static_cast<int>(a.channels), blocks = static_cast<int>(a.tiles_per_row), step = per_row * CODE_BLOCK;
-    const int c0 = sub * CODE_BLOCK + lane_at<VEC>(lane);      // the lane's first channel
-    const int most = (blocks - sub + per_row - 1) / per_row;   // blocks of this warp
-    const auto left_of = [&](int i, int n) { return i < n ? min(CODE_BLOCK - lane_at<VEC>(lane), C - c0 - i * step) : 0; };
-    const auto own_of = [&](int64_t row) { return row < a.outer ? most : 0; };   // a warp without a row still takes part in the sums
-    W next_scale = 0;   // lane i: of the warp's block i
+    Quad<T>* const gy_slot = reinterpret_cast<Quad<T>*>(slots) + threadIdx.x;   // [N][threads] each
+    Quad<T>* const more_slot = gy_slot + N * COUNT;
+    typename Held::Slot* const sum_slot = reinterpret_cast<typename Held::Slot*>(slots + 2 * N * COUNT * sizeof(Quad<T>)) + threadIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = WARPS >> shift;
+    const RowTile<VEC, ROWS, BLOCKS> t(a.channels, a.tiles_per_row, shift, lane, warp);
+    const auto rows_from = [&](int64_t row) { return static_cast<int>(max(int64_t(0), min(static_cast<int64_t>(ROWS), a.outer - row))); };
+    const auto block_of = [&](int64_t row, int q) { return row * a.tiles_per_row + (t.c0 - t.at) / CODE_BLOCK + (static_cast<int64_t>(q) << shift); };
+    W next_scale = 0;   // lane q: of quad q
     const auto fetch = [&](int64_t row) {
-        const int own = own_of(row);
-        const int64_t first = row * C + c0;
+        const int rows = rows_from(row);
+        const int64_t first = row * t.C + t.c0;
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
+        for (int q = 0; q < N; q++)
         {
-            Held::template fetch<VEC>(a, sum_slot + i * COUNT, first + i * step, left_of(i, own));
-            fetch_quad<VEC>(gy_slot + i * COUNT, static_cast<const T*>(a.gy), first + i * step, left_of(i, own));
+            Held::template fetch<VEC>(a, sum_slot + q * COUNT, first + t.offset(q), t.left(q, rows));
+            fetch_quad<VEC>(gy_slot + q * COUNT, static_cast<const T*>(a.gy), first + t.offset(q), t.left(q, rows));
         }
-        if (CODES && lane < min(own, HELD)) next_scale = __ldg(static_cast<const W*>(a.sum_scales) + row * blocks + sub + lane * per_row);
+        if (CODES && rows > 0 && lane < min(t.count(rows), N)) next_scale = __ldg(static_cast<const W*>(a.sum_scales) + block_of(row, lane));
     };
     const auto fetch_more = [&](int64_t row) {
         if (a.gsum == nullptr) return;
+        const int rows = rows_from(row);
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
-            fetch_quad<VEC>(more_slot + i * COUNT, static_cast<const T*>(a.gsum), row * C + c0 + i * step, left_of(i, own_of(row)));
+        for (int q = 0; q < N; q++) fetch_quad<VEC>(more_slot + q * COUNT, static_cast<const T*>(a.gsum), row * t.C + t.c0 + t.offset(q), t.left(q, rows));
     };
-    const int64_t stride = static_cast<int64_t>(gridDim.x) * groups;
-    int64_t row = static_cast<int64_t>(blockIdx.x) * groups + warp / per_row;
+    const auto weights_of = [&](int j, W (&g)[4]) {
+        if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + j * t.step, t.left_in(j)), g);
+        else
+#pragma unroll
+            for (int k = 0; k < 4; k++) g[k] = W(1);
+    };
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * groups * ROWS;
+    int64_t row = (static_cast<int64_t>(blockIdx.x) * groups + (warp >> shift)) * ROWS;
+    int turn = 0;
     if (AHEAD)
     {
         fetch(row);
@@ -864,21 +947,21 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
         fetch_more(row);
         fetch_commit();
     }
-    W weight_sum[HELD][4] = {};
-    for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * groups; row0 < a.outer; row0 += stride, row += stride)
+    W weight_sum[BLOCKS][4] = {};
+    for (; row < a.outer; row += stride)
     {
-        const int own = own_of(row);
-        const int64_t first = row * C + c0;
-        Held s[HELD];
-        Quad<T> gy[HELD];
+        const int rows = rows_from(row), count = t.count(rows);
+        const int64_t first = row * t.C + t.c0;
+        Held s[N];
+        Quad<T> gy[N];
         if (AHEAD)
         {
             fetch_wait<1>();   // gsum may still travel
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int q = 0; q < N; q++)
             {
-                s[i].take(sum_slot[i * COUNT], CODES ? __shfl_sync(0xffffffffu, next_scale, i) : W(0));
-                gy[i] = gy_slot[i * COUNT];
+                s[q].take(sum_slot[q * COUNT], CODES ? __shfl_sync(0xffffffffu, next_scale, q) : W(0));
+                gy[q] = gy_slot[q * COUNT];
             }
             __syncwarp();
             fetch(row + stride);
@@ -886,69 +969,64 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
         }
         else
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int q = 0; q < N; q++)
             {
-                s[i].template load<VEC>(a, first + i * step, row * blocks + sub + i * per_row, left_of(i, own), i < own);
-                gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + first + i * step, left_of(i, own));
+                s[q].template load<VEC>(a, first + t.offset(q), block_of(row, q), t.left(q, rows), q < count);
+                gy[q] = load_quad<VEC>(static_cast<const T*>(a.gy) + first + t.offset(q), t.left(q, rows));
             }
-        const auto weights_of = [&](int i, W (&g)[4]) {
-            if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + c0 + i * step, left_of(i, most)), g);
-            else
-#pragma unroll
-                for (int k = 0; k < 4; k++) g[k] = W(1);
-        };
-        const auto add_up = [&](auto zero, double (&total)[2]) {
+        const auto add_up = [&](auto zero, double (&total)[2]) {   // squares and products of row lane % ROWS
             using A = decltype(zero);
-            A squares = 0, products = 0;
+            A squares[ROWS] = {}, products[ROWS] = {};
+            W g[4];
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int q = 0; q < N; q++)
             {
-                W v[4], up[4], g[4];
-                s[i].values(v);
-                widen_quad(gy[i], up);
-                weights_of(i, g);
+                W v[4], up[4];
+                s[q].values(v);
+                widen_quad(gy[q], up);
+                if (BLOCKS > 1 || q == 0) weights_of(q % BLOCKS, g);
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                 {
-                    squares = fma(static_cast<A>(v[k]), static_cast<A>(v[k]), squares);
-                    products = fma(static_cast<A>(v[k]), static_cast<A>(up[k]) * static_cast<A>(g[k]), products);
+                    squares[q / BLOCKS] = fma(static_cast<A>(v[k]), static_cast<A>(v[k]), squares[q / BLOCKS]);
+                    products[q / BLOCKS] = fma(static_cast<A>(v[k]), static_cast<A>(up[k]) * static_cast<A>(g[k]), products[q / BLOCKS]);
                 }
             }
-            total[0] = group_sum<WARPS>(squares, part, per_row);
-            total[1] = group_sum<WARPS>(products, part, per_row);
+            total[0] = static_cast<double>(spread_sums(squares, lane));
+            total[1] = static_cast<double>(spread_sums(products, lane));
+            share_sums(total, part, turn, shift);
         };
         double total[2];
         add_up(W(0), total);
-        // The warps of a row agree; where rows are shared the thread block decides as one, because its barriers are in common.
-        bool again = sizeof(W) == 4 && out_of_range(total[0], total[1], a.eps);
-        if (per_row > 1) again = __syncthreads_or(again);
-        if (again)
+        if (sizeof(W) == 4 && __any_sync(0xffffffffu, out_of_range(total[0], total[1], a.eps)))   // the warps that share a row agree
         {
             rarely();
             add_up(0.0, total);
         }
         W r, pull;
-        gradient_factors(total[0], total[1], static_cast<double>(C), a.eps, r, pull);
-        if (AHEAD) fetch_wait<1>();   // gsum is here, the next row may travel
+        gradient_factors(total[0], total[1], a.per_channel, a.eps, r, pull);
+        if (AHEAD) fetch_wait<1>();   // gsum is here, the next rows may travel
+        W g[4];
 #pragma unroll
-        for (int i = 0; i < HELD; i++)
+        for (int q = 0; q < N; q++)
         {
-            if (i >= own) break;
+            if (q >= count) break;
             Quad<T> more;
-            if (a.gsum != nullptr) more = AHEAD ? more_slot[i * COUNT] : load_quad<VEC>(static_cast<const T*>(a.gsum) + first + i * step, left_of(i, own));
-            W v[4], up[4], g[4], gx[4];
-            s[i].forget_values();
-            forget_widened(gy[i]);
-            s[i].values(v);
-            widen_quad(gy[i], up);
-            weights_of(i, g);
+            if (a.gsum != nullptr) more = AHEAD ? more_slot[q * COUNT] : load_quad<VEC>(static_cast<const T*>(a.gsum) + first + t.offset(q), t.left(q, rows));
+            W v[4], up[4], gx[4];
+            s[q].forget_values();
+            forget_widened(gy[q]);
+            s[q].values(v);
+            widen_quad(gy[q], up);
+            if (BLOCKS > 1 || q == 0) weights_of(q % BLOCKS, g);
+            const W r_row = ROWS == 1 ? r : __shfl_sync(0xffffffffu, r, q / BLOCKS), pull_row = ROWS == 1 ? pull : __shfl_sync(0xffffffffu, pull, q / BLOCKS);
 #pragma unroll
             for (int k = 0; k < 4; k++)
             {
-                gx[k] = r * (up[k] * g[k] - v[k] * pull);
-                weight_sum[i][k] += up[k] * (v[k] * r);
+                gx[k] = r_row * (up[k] * g[k] - v[k] * pull_row);
+                weight_sum[q % BLOCKS][k] += up[k] * (v[k] * r_row);
             }
-            put_gradient<VEC, 32, T>(a, gx, &more, first + i * step, left_of(i, own));
+            put_gradient<VEC, 32, T>(a, gx, &more, first + t.offset(q), t.left(q, rows));
         }
         if (AHEAD)
         {
@@ -961,21 +1039,21 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
     if (AHEAD) fetch_wait<0>();   // nothing lands in what follows
     __syncthreads();
     W* const weight_sums = reinterpret_cast<W*>(slots);   // [channels]
-    for (int turn = 0; turn < groups; turn++)
+    for (int n = 0; n < groups; n++)
     {
-        if (warp / per_row == turn)
+        if (warp >> shift == n)
 #pragma unroll
-            for (int i = 0; i < HELD; i++)
+            for (int j = 0; j < BLOCKS; j++)
 #pragma unroll
                 for (int k = 0; k < 4; k++)
                 {
-                    const int c = (sub + i * per_row) * CODE_BLOCK + quad_at<VEC>(lane, k);
-                    if (c < C) weight_sums[c] = (turn == 0 ? W(0) : weight_sums[c]) + weight_sum[i][k];
+                    const int c = t.c0 - t.at + j * t.step + quad_at<VEC>(lane, k);
+                    if (j < t.own && c < t.C) weight_sums[c] = (n == 0 ? W(0) : weight_sums[c]) + weight_sum[j][k];
                 }
         __syncthreads();
     }
-    W* const partial = static_cast<W*>(a.partial) + static_cast<int64_t>(blockIdx.x) * C;
-    for (int c = threadIdx.x; c < C; c += WARPS * 32) partial[c] = weight_sums[c];
+    W* const partial = static_cast<W*>(a.partial) + static_cast<int64_t>(blockIdx.x) * t.C;
+    for (int c = threadIdx.x; c < t.C; c += WARPS * 32) partial[c] = weight_sums[c];
 }
 
 /// gweight from the rows of partial sums, in double and in a fixed order: a thread block takes 32 channels and its 32 warps every 32nd row, all of

@@ -11,6 +11,22 @@ struct NormGradArgs;
 template <typename T> int rms_norm_forward(const NormArgs& a, cudaStream_t stream);
 template <typename T> int rms_norm_backward(const NormGradArgs& a, cudaStream_t stream);
 
+/// How rows of channels are dealt out: a thread block of `warps` warps takes `rows` rows at once, 2^shift warps a row, and a warp holds `blocks` blocks
+/// of 128 channels of each of its rows. Rows of one and two blocks go four and two to a warp.
+struct RowSplit
+{
+    int rows, warps, shift, blocks;
+};
+inline RowSplit split_rows(int64_t blocks)
+{
+    if (blocks <= 2) return {blocks == 1 ? 32 : 16, 8, 0, static_cast<int>(blocks)};
+    if (blocks > 64) return {1, 16, 4, 8};
+    if (blocks > 32) return {1, 16, 4, 4};
+    int shift = 0;
+    while (blocks > (4 << shift)) shift++;
+    return {8 >> shift, 8, shift, 4};
+}
+
 /// Thread blocks of the backward kernels, each of which leaves one row of partial sums of gweight. They walk over the tiles (or
 /// rows): more of them than are resident would only add rows.
 inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner, bool wide)
@@ -23,10 +39,8 @@ inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner
         const int64_t pixels = channels <= whole ? 128 : channels <= 2 * whole ? 64 : channels <= held ? 32 : 128;
         return std::min(outer * ((inner + pixels - 1) / pixels), SMS * (channels <= 4 * whole ? 2 : 1));
     }
-    const int64_t blocks = code_blocks(channels);
-    int64_t groups = 8;   // rows that a thread block has at work
-    while (groups > 1 && blocks * groups > 32) groups /= 2;
-    return std::min((outer + groups - 1) / groups, SMS * (blocks > 32 ? 1 : 2));
+    const RowSplit split = split_rows(code_blocks(channels));
+    return std::min((outer + split.rows - 1) / split.rows, SMS * (split.warps == 8 ? 2 : 1));
 }
 
 }  // namespace mc

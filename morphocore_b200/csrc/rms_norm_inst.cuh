@@ -11,6 +11,7 @@ namespace
 {
 
 constexpr int LARGEST_GRID = 0x7fffffff;
+template <int N> using Int = std::integral_constant<int, N>;
 
 /// Launches KERNEL, whose shared memory needs an opt-in where it leaves the first 48 KiB with what the kernel declares itself. The opt-in is asked for
 /// once a device (and again for more): it is 1 us of host time.
@@ -39,14 +40,6 @@ int launch_norm(int64_t grid, int warps, size_t shared, cudaStream_t stream, con
     return check_launch(what);
 }
 
-/// Warps that share a row of `blocks` blocks when each keeps up to `held`: a power of two, at most `most`.
-int warps_per_row(int64_t blocks, int held, int most)
-{
-    int n = 1;
-    while (n < most && blocks > static_cast<int64_t>(n) * held) n *= 2;
-    return n;
-}
-
 template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaStream_t stream)
 {
     constexpr bool WIDE = sizeof(T) == 8, HALF = sizeof(T) == 2;
@@ -54,9 +47,16 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
     constexpr const char* COLUMNS = "rms_norm_columns_kernel";
     if (rows)
     {
-        if (a.tiles_per_row > 32) return launch_norm<rms_norm_rows_kernel<T, VEC, 8, 16, 1>>(a.outer, 16, 0, stream, ROWS, a, 16);
-        const int per_row = warps_per_row(a.tiles_per_row, 4, 8), groups = 8 / per_row;
-        return launch_norm<rms_norm_rows_kernel<T, VEC, 4, 8, WIDE ? 2 : 3>>((a.outer + groups - 1) / groups, 8, 0, stream, ROWS, a, per_row);
+        const RowSplit split = split_rows(a.tiles_per_row);
+        const auto launch = [&](auto rows, auto blocks, auto warps, auto ctas) {
+            return launch_norm<rms_norm_rows_kernel<T, VEC, rows, blocks, warps, ctas>>((a.outer + split.rows - 1) / split.rows, warps, 0, stream, ROWS, a, split.shift);
+        };
+        constexpr Int<WIDE ? 2 : 4> CTAS;
+        if (split.blocks == 1) return launch(Int<4>(), Int<1>(), Int<8>(), CTAS);
+        if (split.blocks == 2) return launch(Int<2>(), Int<2>(), Int<8>(), CTAS);
+        if (split.blocks == 8) return launch(Int<1>(), Int<8>(), Int<16>(), Int<1>());
+        if (split.warps == 8) return launch(Int<1>(), Int<4>(), Int<8>(), CTAS);
+        return launch(Int<1>(), Int<4>(), Int<16>(), Int<WIDE ? 1 : 2>());
     }
     if (a.channels <= 32) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 8, 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
     if constexpr (WIDE) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 16, 1>>(a.tiles, 16, 0, stream, COLUMNS, a);   // eight quads of doubles do not fit
@@ -76,12 +76,19 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
     if (rows)
     {
         // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
-        constexpr size_t MANY = gradient_slot_bytes<T, CODES>(8, 512);
-        constexpr bool FITS = MANY <= 200 * 1024;
-        if (a.tiles_per_row > 32)
-            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, FITS, 8, 16, 1>>(grid, 16, std::max(FITS ? MANY : 0, sums), stream, ROWS, a, 16);
-        return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, true, 4, 8, 2>>(grid, 8, std::max(FEW, sums), stream, ROWS, a,
-                                                                                       warps_per_row(a.tiles_per_row, 4, 8));
+        constexpr bool FITS = gradient_slot_bytes<T, CODES>(8, 512) <= 200 * 1024;
+        const RowSplit split = split_rows(a.tiles_per_row);
+        const auto launch = [&](auto ahead, auto rows, auto blocks, auto warps, auto ctas) {
+            const size_t slots = ahead ? gradient_slot_bytes<T, CODES>(rows * blocks, warps * 32) : 0;
+            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
+                                                                                                              split.shift);
+        };
+        constexpr std::true_type AHEAD;
+        if (split.blocks == 1) return launch(AHEAD, Int<4>(), Int<1>(), Int<8>(), Int<2>());
+        if (split.blocks == 2) return launch(AHEAD, Int<2>(), Int<2>(), Int<8>(), Int<2>());
+        if (split.blocks == 8) return launch(std::bool_constant<FITS>(), Int<1>(), Int<8>(), Int<16>(), Int<1>());
+        if (split.warps == 8) return launch(AHEAD, Int<1>(), Int<4>(), Int<8>(), Int<2>());
+        return launch(AHEAD, Int<1>(), Int<4>(), Int<16>(), Int<1>());
     }
     constexpr size_t MORE = gradient_slot_bytes<T, CODES>(8, 256);
     if (a.channels <= 32) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 1, 2>>(grid, 8, FEW, stream, COLUMNS, a);
