@@ -167,8 +167,8 @@ __device__ __forceinline__ void put_codes(int8_t* codes, void* scales, Offset of
 // The kernels that keep a tile in registers fetch the next one meanwhile, by asynchronous copies into slots of shared memory that only
 // the thread that issued the copy reads: no barrier and no register is spent on it, and the loads of one tile travel while the sums,
 // barriers and stores of another take their time. A slot may be fetched into again once its reader has passed a __syncwarp.
-// Backward, float, (32, 64, 224, 224): 272 us against 304 without; bfloat16 (16, 128, 112, 112): 55 against 70; bfloat16 (65536, 512) rows:
-// 75 against 103. Rows that need copies of single elements lose a little ((40, 20, 75, 101): 40 against 33). The forward kernels do not
+// Backward, float, (32, 64, 224, 224): 272 us against 304 without; bfloat16 (65536, 512) rows: 75 against 103. Rows that need copies of single
+// elements lose a little ((40, 20, 75, 101): 40 against 33). The forward kernels do not
 // fetch ahead: with a residual it cost 45 us of 247, because thread blocks that stay drift apart, and neighbouring tiles, which share
 // pages of memory, are then no longer read together.
 
@@ -293,20 +293,20 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
             return total;
         };
         __syncthreads();
-        double total = 0.0;
-        if (threadIdx.x < CODE_BLOCK) total = put_factor();
+        bool again = false;
+        if (threadIdx.x < CODE_BLOCK) again = out_of_range(put_factor(), 0.0, a.eps);
         if (sizeof(Sum<T>) == 8) __syncthreads();
-        else if (__syncthreads_or(out_of_range(total, 0.0, a.eps)))
+        else if (__syncthreads_or(again))   // for the pixels that need it: no result depends on what its neighbours hold
         {
-            double again[4] = {};
+            double exact[4] = {};
             for (int i0 = 0; i0 < own; i0 += HELD)
             {
                 if (!held) load(a.residual != nullptr ? a.sum : a.x, i0, s);
-                add_squares(s, again);
+                add_squares(s, exact);
             }
-            put_sums(again);
+            put_sums(exact);
             __syncthreads();
-            if (threadIdx.x < CODE_BLOCK) put_factor();
+            if (again) put_factor();
             __syncthreads();
         }
         Factor<T> r[4];
@@ -347,9 +347,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
                     else
                     {
                         rarely();
+                        times(v, r[0], r[1], r[2], r[3], weights, result);
 #pragma unroll
                         for (int k = 0; k < 4; k++)
-                            result[k] = static_cast<W>(static_cast<double>(v[k]) * factor[quad_at<VEC>(lane, k)] * static_cast<double>(g[i]));
+                        {
+                            const double exact = factor[quad_at<VEC>(lane, k)];
+                            if (!ordinary(exact) || !ordinary_weight(g[i])) result[k] = static_cast<W>(static_cast<double>(v[k]) * exact * static_cast<double>(g[i]));
+                        }
                     }
                     y[i] = narrow_quad<T>(result);
                 }
@@ -404,7 +408,7 @@ template <int K, int WARPS> __device__ __forceinline__ void share_sums(double (&
 
 /// How a warp of the kernels for rows of channels holds ROWS neighbouring rows of BLOCKS blocks of 128 channels each; 2^shift warps share a row, warp
 /// `sub` of them has the blocks sub, sub + 2^shift, ... More than one row is for rows of exactly BLOCKS blocks that no warps share. Without that a row
-/// of few channels leaves most of what a warp is unrolled for empty: (65536, 64) in float took 45 us, ROWS_FEW so.
+/// of few channels leaves most of what a warp is unrolled for empty: (65536, 64) in float took 45 us forward and 56 backward, 11 and 23 so.
 template <bool VEC, int ROWS, int BLOCKS> struct RowTile
 {
     int C, c0, own, step, at;   // channels; the lane's first; blocks of this warp; channels from one to the next; the lane's place in a block
@@ -424,7 +428,8 @@ template <bool VEC, int ROWS, int BLOCKS> struct RowTile
     __device__ __forceinline__ int count(int rows) const { return ROWS == 1 ? own : rows * BLOCKS; }
 };
 
-/// Forward, rows of channels.
+/// Forward, rows of channels. Bytes bound it in float: (32768, 1024) 84 us with the residual, 97 % of the copy rate, 70 with codes. In half precision
+/// instructions do, some 20 an element ((65536, 512) bfloat16 38 us, 53 %; with residual 49, 83 %). Four thread blocks an SM: three take 43 and 62 us there.
 template <typename T, bool VEC, int ROWS, int BLOCKS, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int shift)
 {
@@ -487,20 +492,26 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
             }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
         double total = add_up(Sum<T>(0));
-        // Squares that left the range of float, or would where eps does not cover them: in double. The warps that share a row agree.
-        if (sizeof(Sum<T>) == 4 && __any_sync(0xffffffffu, out_of_range(total, 0.0, a.eps)))
+        // Squares that left the range of float, or would where eps does not cover them: in double. The warps that share a row agree, and the rows
+        // that share a warp stay as they are without one another.
+        const bool again = sizeof(Sum<T>) == 4 && out_of_range(total, 0.0, a.eps);
+        if (__any_sync(0xffffffffu, again))
         {
             rarely();
-            total = add_up(0.0);
+            const double exact = add_up(0.0);
+            if (again) total = exact;
         }
         const double factor = norm_factor(total, a.per_channel, a.eps);
-        const bool all_ordinary = __all_sync(0xffffffffu, ordinary(factor));
+        // Bit i: row i. One row as a yes or no of the whole warp, which the compiler turns into a branch around the loop below (50 us against 56 for
+        // (65536, 512) bfloat16 with residual).
+        const unsigned ordinary_rows = ROWS == 1 ? __all_sync(0xffffffffu, ordinary(factor)) : __ballot_sync(0xffffffffu, ordinary(factor));
+        const bool some_ordinary = ordinary_rows != 0;
         Factor<T> mine, r[ROWS];
         mine.set(factor);
 #pragma unroll
         for (int i = 0; i < ROWS; i++) r[i] = ROWS == 1 ? mine : mine.of_lane(i);
         W g[4] = {1, 1, 1, 1};
-        bool usual = all_ordinary;
+        bool usual = some_ordinary;
 #pragma unroll
         for (int g0 = 0; g0 < N; g0 += GROUP)
         {
@@ -515,10 +526,10 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
                 if (a.weight != nullptr && (BLOCKS > 1 || q == 0))
                 {
                     widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + q % BLOCKS * t.step, t.left_in(q % BLOCKS)), g);
-                    usual = all_ordinary && __all_sync(0xffffffffu, ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]));
+                    usual = some_ordinary && __all_sync(0xffffffffu, ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]));
                 }
                 const Factor<T>& f = r[q / BLOCKS];
-                if (usual) times(v, f, f, f, f, g, result);
+                if (usual && (ROWS == 1 || (ordinary_rows >> (q / BLOCKS) & 1u) != 0)) times(v, f, f, f, f, g, result);
                 else   // the whole warp
                 {
                     rarely();
@@ -628,9 +639,10 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
         part[1][group][quad_at<VEC, LANES>(lane, k)] = sums[1][k];
     }
     __syncthreads();
-    double total[2] = {};
+    bool again = false;
     if (threadIdx.x < PIXELS)
     {
+        double total[2] = {};
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
         {
@@ -638,12 +650,13 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
             total[1] += static_cast<double>(part[1][g][threadIdx.x]);
         }
         gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        again = out_of_range(total[0], total[1], eps);
     }
     if constexpr (sizeof(W) == 8) __syncthreads();
-    else if (__syncthreads_or(threadIdx.x < PIXELS && out_of_range(total[0], total[1], eps)))
+    else if (__syncthreads_or(again))   // for the pixels that need it: no result depends on what its neighbours hold
     {
         rarely();
-        double exact[2][4] = {};
+        double exact[2][4] = {}, total[2] = {};
         add_up(exact);
         double(*const wide)[PIXELS] = reinterpret_cast<double(*)[PIXELS]>(&part[0][0][0]);   // [GROUPS][PIXELS]
         for (int q = 0; q < 2; q++)
@@ -651,14 +664,11 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
 #pragma unroll
             for (int k = 0; k < 4; k++) wide[group][quad_at<VEC, LANES>(lane, k)] = q == 0 ? exact[0][k] : exact[1][k];
             __syncthreads();
-            if (threadIdx.x < PIXELS)
-            {
-                total[q] = 0.0;
+            if (again)
                 for (int g = 0; g < GROUPS; g++) total[q] += wide[g][threadIdx.x];
-            }
             __syncthreads();
         }
-        if (threadIdx.x < PIXELS) gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        if (again) gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
         __syncthreads();
     }
 }
@@ -998,10 +1008,17 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
         };
         double total[2];
         add_up(W(0), total);
-        if (sizeof(W) == 4 && __any_sync(0xffffffffu, out_of_range(total[0], total[1], a.eps)))   // the warps that share a row agree
+        const bool again = sizeof(W) == 4 && out_of_range(total[0], total[1], a.eps);   // the warps that share a row agree
+        if (__any_sync(0xffffffffu, again))
         {
             rarely();
-            add_up(0.0, total);
+            double exact[2];
+            add_up(0.0, exact);
+            if (again)
+            {
+                total[0] = exact[0];
+                total[1] = exact[1];
+            }
         }
         W r, pull;
         gradient_factors(total[0], total[1], a.per_channel, a.eps, r, pull);

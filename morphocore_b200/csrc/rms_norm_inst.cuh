@@ -58,11 +58,12 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
         if (split.warps == 8) return launch(Int<1>(), Int<4>(), Int<8>(), CTAS);
         return launch(Int<1>(), Int<4>(), Int<16>(), Int<WIDE ? 1 : 2>());
     }
-    if (a.channels <= 32) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 8, 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
-    if constexpr (WIDE) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 16, 1>>(a.tiles, 16, 0, stream, COLUMNS, a);   // eight quads of doubles do not fit
-    else
+    // Thread blocks an SM: as many as the registers of a tile let in without spilling it. Eight quads of doubles do not fit at all: two thread blocks that
+    // read 33 to 64 channels again from L2 take 50 to 80 us for (16, 64, 112, 112) where one of 16 warps that keeps them takes 62 to 91.
+    if (WIDE || a.channels <= 32) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 8, HALF ? 3 : 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
+    if constexpr (!WIDE)
     {
-        if (a.channels <= 64) return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 8, HALF ? 3 : 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
+        if (a.channels <= 64) return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 8, !HALF ? 2 : VEC ? 4 : 3>>(a.tiles, 8, 0, stream, COLUMNS, a);
         return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 16, HALF ? 2 : 1>>(a.tiles, 16, 0, stream, COLUMNS, a);
     }
 }

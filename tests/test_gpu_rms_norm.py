@@ -122,6 +122,40 @@ def test_gradients(shape, dim, dtype, keep8):
             within(got[1], want_w, weight_bound(size_w, want_w, dtype, channels=shape[dim]), "weight")
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("rows,channels", [(1, 3), (2, 64), (34, 20), (67, 127), (3, 128), (1, 129), (18, 200), (33, 256), (3, 257), (9, 600), (5, 1500), (3, 4095), (2, 8192),
+                                           (2, 9001)], ids=str)
+def test_rows_that_share_warps_and_warps_that_share_rows(rows, channels, dtype):
+    test_forward_and_codes((rows, channels), -1, dtype)
+    for keep8 in (False, True):
+        test_gradients((rows, channels), -1, dtype, keep8)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,dim", [((35, 40), -1), ((35, 128), -1), ((19, 250), -1), ((5, 700), -1), ((21, 700), -1), ((2, 9, 13, 12), -3), ((2, 70, 13, 11), -3), ((1, 600, 6, 6), -3)], ids=str)
+def test_nothing_of_a_neighbour(shape, dim, dtype):
+    """Rows, and pixels, that leave the range of float, hold infinities or NaN, change not one bit of the others."""
+    info = torch.finfo(dtype)
+    results = []
+    for special in (False, True):
+        s = make(shape, dtype, 6)
+        pixels = s.transpose(dim, -1).reshape(-1, s.shape[dim]).clone()
+        others = torch.ones(len(pixels), dtype=torch.bool)
+        for i, value in enumerate((info.max, float("inf"), info.smallest_normal, float("nan"), 0.0)):
+            others[2 * i % len(pixels)::10] = False
+            if special:
+                pixels[2 * i % len(pixels)::10] = value
+        wide = list(s.shape)
+        wide[dim], wide[-1] = wide[-1], wide[dim]
+        x = pixels.reshape(wide).transpose(dim, -1).contiguous().cuda().requires_grad_(True)
+        w = make((shape[dim],), dtype, 3, 0.2, 1.0).cuda()
+        y = F.rms_norm(x, w, eps=1e-30, dim=dim)
+        gx, = torch.autograd.grad(y, x, make(shape, dtype, 4).cuda())
+        results.append([t.detach().cpu().transpose(dim, -1).reshape(-1, s.shape[dim])[others] for t in (y, gx)])
+    for usual, beside in zip(*results):
+        assert bool((usual == beside).all())
+
+
 @pytest.mark.parametrize("shape,dim", [((40, 24, 60, 60), -3), ((24, 65, 64, 64), -3), ((6, 200, 72, 72), -3), ((60000, 48), -1), ((9000, 520), -1), ((700, 4100), -1)], ids=str)
 @pytest.mark.parametrize("keep8", [False, True])
 def test_more_tiles_than_thread_blocks(shape, dim, keep8):
