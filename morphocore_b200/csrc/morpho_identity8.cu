@@ -38,8 +38,7 @@ Identity8Args common(const mc_desc& d)
 
 /// Strips of the backward kernel. A strip of r rows takes r + K - 1 steps, and the warps of all strips come in waves of what is resident: the strips
 /// of at least 8 rows with the fewest steps in all. ((16, 64, 112, 112) at 3 x 3: three strips a plane, a few more than are resident at once,
-/// took 125 us where two take 78.)
-/// False where there are more of them than can be counted.
+/// took 125 us where two take 78.) False where there are more of them than can be counted.
 bool set_strips(Identity8Args& a, const mc_desc& d)
 {
     const int64_t planes = static_cast<int64_t>(d.B) * d.Ci;
@@ -47,7 +46,7 @@ bool set_strips(Identity8Args& a, const mc_desc& d)
     const int64_t columns = planes * a.column_tiles, resident = 148 * (d.kH == 3 ? BACKWARD_WARPS_3 : BACKWARD_WARPS_5) * (32 / strip_lanes(d.W));
     const int extra = d.kH - 1;
     int64_t best = 0;
-    for (int strips = 1; strips <= std::max(1, d.H / 8); strips++)
+    for (int strips = 1; strips <= std::max(1, d.H / 8); strips += 1 + strips / 64)   // not every number of them in a tall image: this is host time
     {
         const int rows = (d.H + strips - 1) / strips, count = (d.H + rows - 1) / rows;
         const int64_t cost = (columns * count + resident - 1) / resident * (rows + extra);

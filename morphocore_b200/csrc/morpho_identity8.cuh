@@ -264,8 +264,8 @@ template <bool IS_MIN, int K, int WARPS> __global__ void __launch_bounds__(32, W
             for (int k = TAPS - 2; k >= 0; k--) at = v[k] == m ? ((k / K) * COLS + k % K) * 128u : at;
             off[j] = m == INITIAL ? 0u : at;
         }
-        // gx: slot of (i, c) = ((step + i) % K) * COLS + c, i = K-1-kh, c = j + K-1-kw; kept as a rolling array shifted every row instead of a ring
-        // `top` is where row h + R lies in the ring, the one below it at the place before; a winner's row is kh places up.
+        // `top` is where row h + R lies in the ring of rows of gx; the row that tap (kh, kw) reads lies kh places before it, its column K - 1 - kw
+        // after the output's.
 #pragma unroll
         for (int j = 0; j < 4; j++)
         {
