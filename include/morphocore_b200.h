@@ -209,7 +209,7 @@ int mc_morpho_backward8(const mc_desc* desc, const int8_t* codes, const void* sc
  * Tensors are [outer, channels, inner], contiguous: (N, C, H * W) for feature maps, (tokens, C, 1) for rows of channels. With
  * s = x + residual rounded to the tensors' type (s = x where there is no residual),
  *     y = s * r * weight[c], r = 1 / sqrt(mean over the channels of s^2 + eps),
- * the sum, the mean and r held in double (for F16 and BF16 the sum and r in float). y and the 8-bit forms are optional (NULL), at least one output is not. The 8-bit form is that of
+ * the mean and r held in double and y rounded once. y and the 8-bit forms are optional (NULL), at least one output is not. The 8-bit form is that of
  * mc_encode8 applied to y, or to s, with rows of `inner` elements, or of `channels` where inner is 1: it is what a layer behind
  * the norm, or the norm itself, may keep for its backward pass instead of the tensor.
  * `sum` receives s; it is required with a residual and must be NULL without. Buffers that are read may not overlap those

@@ -87,8 +87,7 @@ int mc_rms_norm_forward(const mc_norm_desc* desc, const void* x, const void* res
 size_t mc_rms_norm_backward_workspace_bytes(const mc_norm_desc* desc, int have_gweight)
 {
     if (!have_gweight || checked_norm(desc) != MC_OK || desc->outer * desc->inner == 0) return 0;
-    const bool wide = desc->dtype == MC_F64;
-    return (wide ? 8 : 4) * static_cast<size_t>(norm_backward_grid(desc->outer, desc->channels, desc->inner, wide)) * static_cast<size_t>(desc->channels);
+    return (desc->dtype == MC_F64 ? 8 : 4) * static_cast<size_t>(norm_backward_grid(desc->outer, desc->channels, desc->inner, element_bytes(*desc))) * static_cast<size_t>(desc->channels);
 }
 
 int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t* sum_codes, const void* sum_scales, const void* weight, const void* gy,

@@ -8,10 +8,10 @@
 // rows of channels (rows), stays in registers between the sums over the channels and what is computed from them. Bytes bound
 // them: a forward pass with residual moves 16 bytes an element in float (13 with the result in 8 bits), a backward pass 16 (13).
 //
-// In float the sums over the channels are taken in double and y is rounded once, from an unevaluated sum of two floats that carries
-// about 46 bits: y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
-// in whatever order (a float that is one unit off moves one code in 10^5 to its neighbour). In half precision both are plain float:
-// what is left of its three half steps after the rounding to 8 or 11 bits is one result in 2^13 or 2^10 that goes to the other neighbour.
+// The forward pass takes the sums over the channels in double and rounds y once, from an unevaluated sum of two floats that carries
+// about 46 bits (from double in double): y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
+// in whatever order. A float that is one unit off moves one code in 10^5 to its neighbour; plain float arithmetic behind a result of 11 bits
+// moves one result in 2^10, and with the largest of a block its scale ((32, 64, 224, 224) in bfloat16 98 us so, 111 as it is).
 #pragma once
 #include <type_traits>
 
@@ -41,19 +41,13 @@ struct NormGradArgs
     double eps, per_channel;
 };
 
-/// What the forward kernels add squares up in.
-template <typename T> struct SumOf { using type = double; };
-template <> struct SumOf<__half> { using type = float; };
-template <> struct SumOf<__nv_bfloat16> { using type = float; };
-template <typename T> using Sum = typename SumOf<T>::type;
-
 /// The factor r of a lane's elements as the products with it are taken, for an ordinary r: the halves are normal floats, and an
-/// infinite s cannot meet them (its r is 0). `times` rounds s r g once to float for float (r as two floats with about 48 bits of it,
-/// pairs of elements by packed instructions) and after each product otherwise.
-template <typename T> struct Factor
+/// infinite s cannot meet them (its r is 0). `times` rounds s r g once to float where that is the wide type (r as two floats with about 48 bits of it,
+/// pairs of elements by packed instructions) and after each product in double.
+template <typename W> struct Factor
 {
-    Wide<T> r;
-    __device__ __forceinline__ void set(double v) { r = static_cast<Wide<T>>(v); }
+    W r;
+    __device__ __forceinline__ void set(double v) { r = v; }
     __device__ __forceinline__ Factor of_lane(int i) const { return {__shfl_sync(0xffffffffu, r, i)}; }
 };
 template <> struct Factor<float>
@@ -67,10 +61,10 @@ template <> struct Factor<float>
     __device__ __forceinline__ Factor of_lane(int i) const { return {__shfl_sync(0xffffffffu, r, i), __shfl_sync(0xffffffffu, low, i)}; }
 };
 
-template <typename T> __device__ __forceinline__ void times(const Wide<T> (&s)[4], const Factor<T>& r0, const Factor<T>& r1, const Factor<T>& r2,
-                                                            const Factor<T>& r3, const Wide<T> (&g)[4], Wide<T> (&y)[4])
+template <typename W>
+__device__ __forceinline__ void times(const W (&s)[4], const Factor<W>& r0, const Factor<W>& r1, const Factor<W>& r2, const Factor<W>& r3, const W (&g)[4], W (&y)[4])
 {
-    if constexpr (std::is_same<T, float>::value)
+    if constexpr (std::is_same<W, float>::value)
     {
         const auto pair = [](float s0, float s1, const Factor<float>& a, const Factor<float>& b, float g0, float g1, float& y0, float& y1) {
             const float2 v = make_float2(s0, s1), g = make_float2(g0, g1);
@@ -136,8 +130,8 @@ template <typename T> __device__ __forceinline__ Quad<T> add_quads(const Quad<T>
     return narrow_quad<T>(u);
 }
 
-/// Sums of squares of N quads, one, two or four for a lane's four elements, added to `sums`.
-template <int N, int SUMS, typename T, typename S> __device__ __forceinline__ void add_squares(const Quad<T> (&s)[N], S (&sums)[SUMS])
+/// Sums of squares of N quads, one or four for a lane's four elements, added to `sums`.
+template <int N, int SUMS, typename T> __device__ __forceinline__ void add_squares(const Quad<T> (&s)[N], double (&sums)[SUMS])
 {
 #pragma unroll
     for (int i = 0; i < N; i++)
@@ -145,7 +139,7 @@ template <int N, int SUMS, typename T, typename S> __device__ __forceinline__ vo
         Wide<T> v[4];
         widen_quad(s[i], v);
 #pragma unroll
-        for (int k = 0; k < 4; k++) sums[k % SUMS] = fma(static_cast<S>(v[k]), static_cast<S>(v[k]), sums[k % SUMS]);
+        for (int k = 0; k < 4; k++) sums[k % SUMS] = fma(static_cast<double>(v[k]), static_cast<double>(v[k]), sums[k % SUMS]);
     }
 }
 
@@ -225,11 +219,11 @@ template <bool VEC, typename Args> __device__ __forceinline__ Place place_of(con
 }
 
 /// Forward, feature maps. A block of WARPS warps takes 128 pixels of an image; warp w has the channels w, w + WARPS, ... and keeps
-/// up to HELD of them. Where there are more, the second pass reads s again, from `sum` or x: the tiles that are at work then
+/// up to eight of them. Where there are more, the second pass reads s again, from `sum` or x: the tiles that are at work then
 /// lie in L2 (128 pixels of 512 channels in float are 256 KiB, of 296 thread blocks 76 MiB).
-template <typename T, bool VEC, int HELD, int WARPS, int CTAS>
-__global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
+template <typename T, bool VEC, int WARPS, int CTAS> __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
 {
+    constexpr int HELD = 8;
     static_assert(WARPS >= 4 && HELD % GROUP == 0, "a thread for every pixel of the tile");
     using W = Wide<T>;
     __shared__ double part[WARPS][CODE_BLOCK];
@@ -251,7 +245,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
 #pragma unroll
             for (int i = 0; i < HELD; i++, p += step) q[i] = load_quad<VEC>(p, i0 + i < own ? left : 0);
         };
-        Sum<T> sums[4] = {};
+        double sums[4] = {};
         for (int i0 = 0; i0 < own; i0 += HELD)
         {
             load(a.x, i0, s);
@@ -279,37 +273,18 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(cons
                 }
         }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
-        // Squares that left the range of float (half precision only), or would where eps does not cover them: in double.
-        const auto put_sums = [&](auto& from) {
 #pragma unroll
-            for (int k = 0; k < 4; k++) part[warp][quad_at<VEC>(lane, k)] = static_cast<double>(from[k]);
-        };
-        put_sums(sums);
-        const auto put_factor = [&]() {
+        for (int k = 0; k < 4; k++) part[warp][quad_at<VEC>(lane, k)] = sums[k];
+        __syncthreads();
+        if (threadIdx.x < CODE_BLOCK)
+        {
             double total = 0.0;
 #pragma unroll
             for (int w = 0; w < WARPS; w++) total += part[w][threadIdx.x];
             factor[threadIdx.x] = norm_factor(total, a.per_channel, a.eps);
-            return total;
-        };
-        __syncthreads();
-        bool again = false;
-        if (threadIdx.x < CODE_BLOCK) again = out_of_range(put_factor(), 0.0, a.eps);
-        if (sizeof(Sum<T>) == 8) __syncthreads();
-        else if (__syncthreads_or(again))   // for the pixels that need it: no result depends on what its neighbours hold
-        {
-            double exact[4] = {};
-            for (int i0 = 0; i0 < own; i0 += HELD)
-            {
-                if (!held) load(a.residual != nullptr ? a.sum : a.x, i0, s);
-                add_squares(s, exact);
-            }
-            put_sums(exact);
-            __syncthreads();
-            if (again) put_factor();
-            __syncthreads();
         }
-        Factor<T> r[4];
+        __syncthreads();
+        Factor<W> r[4];
         bool all_ordinary = true;
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -429,7 +404,8 @@ template <bool VEC, int ROWS, int BLOCKS> struct RowTile
 };
 
 /// Forward, rows of channels. Bytes bound it in float: (32768, 1024) 84 us with the residual, 97 % of the copy rate, 70 with codes. In half precision
-/// instructions do, some 20 an element ((65536, 512) bfloat16 38 us, 53 %; with residual 49, 83 %). Four thread blocks an SM: three take 43 and 62 us there.
+/// instructions do, some 20 an element: (65536, 512) in bfloat16 44 us, with residual 53 (77 %). Four thread blocks an SM: three take 48 and 58, five
+/// spill (48 and 64).
 template <typename T, bool VEC, int ROWS, int BLOCKS, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int shift)
 {
@@ -462,21 +438,6 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
                 store_quad<VEC>(static_cast<T*>(a.sum) + first + t.offset(i), s[i], t.left(i, rows));
             }
         }
-        const auto add_up = [&](auto zero) {   // the squares of row lane % ROWS
-            decltype(zero) sums[ROWS][2] = {};
-#pragma unroll
-            for (int i = 0; i < N; i++)
-            {
-                const Quad<T> one[1] = {s[i]};
-                add_squares(one, sums[i / BLOCKS]);
-            }
-            decltype(zero) own[ROWS];
-#pragma unroll
-            for (int i = 0; i < ROWS; i++) own[i] = sums[i][0] + sums[i][1];
-            double total[1] = {static_cast<double>(spread_sums(own, lane))};
-            share_sums(total, part, turn, shift);
-            return total[0];
-        };
         const auto put = [&](int8_t* codes, void* scales, const Quad<T> (&q)[GROUP], int g0) {
             const int lefts[GROUP] = {t.left(g0, rows), t.left(g0 + 1, rows), t.left(g0 + 2, rows), t.left(g0 + 3, rows)};
             put_codes<VEC>(codes + first, static_cast<W*>(scales) + first_block + (static_cast<int64_t>(g0) << shift), [&](int i) { return t.offset(g0 + i); },
@@ -491,22 +452,23 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
                 put(a.sum_codes, a.sum_scales, q, g0);
             }
         if (a.y == nullptr && a.y_codes == nullptr) continue;
-        double total = add_up(Sum<T>(0));
-        // Squares that left the range of float, or would where eps does not cover them: in double. The warps that share a row agree, and the rows
-        // that share a warp stay as they are without one another.
-        const bool again = sizeof(Sum<T>) == 4 && out_of_range(total, 0.0, a.eps);
-        if (__any_sync(0xffffffffu, again))
+        double squares[ROWS][1] = {}, own[ROWS];
+#pragma unroll
+        for (int i = 0; i < N; i++)
         {
-            rarely();
-            const double exact = add_up(0.0);
-            if (again) total = exact;
+            const Quad<T> one[1] = {s[i]};
+            add_squares(one, squares[i / BLOCKS]);
         }
-        const double factor = norm_factor(total, a.per_channel, a.eps);
+#pragma unroll
+        for (int i = 0; i < ROWS; i++) own[i] = squares[i][0];
+        double total[1] = {spread_sums(own, lane)};   // of row lane % ROWS
+        share_sums(total, part, turn, shift);
+        const double factor = norm_factor(total[0], a.per_channel, a.eps);
         // Bit i: row i. One row as a yes or no of the whole warp, which the compiler turns into a branch around the loop below (50 us against 56 for
         // (65536, 512) bfloat16 with residual).
         const unsigned ordinary_rows = ROWS == 1 ? __all_sync(0xffffffffu, ordinary(factor)) : __ballot_sync(0xffffffffu, ordinary(factor));
         const bool some_ordinary = ordinary_rows != 0;
-        Factor<T> mine, r[ROWS];
+        Factor<W> mine, r[ROWS];
         mine.set(factor);
 #pragma unroll
         for (int i = 0; i < ROWS; i++) r[i] = ROWS == 1 ? mine : mine.of_lane(i);
@@ -528,7 +490,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
                     widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + q % BLOCKS * t.step, t.left_in(q % BLOCKS)), g);
                     usual = some_ordinary && __all_sync(0xffffffffu, ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]));
                 }
-                const Factor<T>& f = r[q / BLOCKS];
+                const Factor<W>& f = r[q / BLOCKS];
                 if (usual && (ROWS == 1 || (ordinary_rows >> (q / BLOCKS) & 1u) != 0)) times(v, f, f, f, f, g, result);
                 else   // the whole warp
                 {
@@ -705,9 +667,10 @@ template <typename T, bool CODES> constexpr size_t gradient_slot_bytes(int held,
 }
 
 /// Backward, feature maps of up to HELD * WARPS * SPLIT channels. A tile is 128 / SPLIT pixels of an image; SPLIT groups of lanes of a warp have
-/// channels of their own, so that a thread block of few warps holds many channels and two of them, which hide each other's barriers, stay
+/// channels of their own, so that a thread block of few warps holds many channels and several of them, which hide each other's barriers, stay
 /// resident. Tiles of 32 pixels, read once, against whole ones read twice: (64, 256, 56, 56) 144 us against 170, (64, 512, 28, 28) 97 against
-/// 118; of 64 pixels in thread blocks of 8 warps against whole ones in 16: (16, 128, 112, 112) 78 against 82. The thread blocks walk over the tiles with
+/// 118. Three thread blocks of 4 warps with tiles of 64 pixels against two of 8 with whole ones: (32, 64, 224, 224) 257 us against 268, from codes 219
+/// against 245; in half precision, four against two: (64, 32, 112, 112) 48 against 50, from codes 50 against 57. The thread blocks walk over the tiles with
 /// gweight's sums in registers; what they have at the end leaves as one row of partial sums, which norm_weight_kernel adds up in a fixed order.
 template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int SPLIT, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_kernel(const NormGradArgs a)
@@ -1073,8 +1036,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
     for (int c = threadIdx.x; c < t.C; c += WARPS * 32) partial[c] = weight_sums[c];
 }
 
-/// gweight from the rows of partial sums, in double and in a fixed order: a thread block takes 32 channels and its 32 warps every 32nd row, all of
-/// which (296 at most) are in flight at once. 7.1 us with 8 warps on 444 rows of 512 channels, 4.3 us so.
+/// gweight from the rows of partial sums, in double and in a fixed order: a thread block takes 32 channels and its 32 warps every 32nd row, many
+/// of which (592 rows at most) are in flight at once. 7.1 us with 8 warps on 444 rows of 512 channels, 4.3 us so.
 constexpr int WEIGHT_WARPS = 32;
 template <typename T>
 __global__ void __launch_bounds__(WEIGHT_WARPS * 32) norm_weight_kernel(const Wide<T>* __restrict__ partial, T* __restrict__ gweight, int64_t channels, int rows)

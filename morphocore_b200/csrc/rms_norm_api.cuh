@@ -27,17 +27,22 @@ inline RowSplit split_rows(int64_t blocks)
     return {8 >> shift, 8, shift, 4};
 }
 
+/// Thread blocks an SM of the backward kernel for feature maps of up to 128 channels, whose elements have this many bytes: as many as its registers let in
+/// without spilling them.
+constexpr int gradient_blocks_per_sm(int element) { return element == 8 ? 2 : element == 4 ? 3 : 4; }
+
 /// Thread blocks of the backward kernels, each of which leaves one row of partial sums of gweight. They walk over the tiles (or
-/// rows): more of them than are resident would only add rows.
-inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner, bool wide)
+/// rows): more of them than are resident would only add rows. `element`: bytes of one.
+inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner, int element)
 {
     constexpr int64_t SMS = 148;
     if (inner != 1)
     {
-        // As the launches choose: the pixels of a tile, and one or two thread blocks an SM.
-        const int64_t whole = wide ? 32 : 64, held = wide ? 128 : 512;
-        const int64_t pixels = channels <= whole ? 128 : channels <= 2 * whole ? 64 : channels <= held ? 32 : 128;
-        return std::min(outer * ((inner + pixels - 1) / pixels), SMS * (channels <= 4 * whole ? 2 : 1));
+        // As the launches choose: the pixels of a tile, and the thread blocks an SM.
+        const int64_t held = element == 8 ? 128 : 512;
+        const int64_t pixels = channels <= 32 ? 128 : channels <= 64 ? 64 : channels <= held ? 32 : 128;
+        const int64_t resident = channels <= 128 ? gradient_blocks_per_sm(element) : channels <= 256 && element < 8 ? 2 : 1;
+        return std::min(outer * ((inner + pixels - 1) / pixels), SMS * resident);
     }
     const RowSplit split = split_rows(code_blocks(channels));
     return std::min((outer + split.rows - 1) / split.rows, SMS * (split.warps == 8 ? 2 : 1));

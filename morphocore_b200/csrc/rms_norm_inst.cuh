@@ -58,14 +58,15 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
         if (split.warps == 8) return launch(Int<1>(), Int<4>(), Int<8>(), CTAS);
         return launch(Int<1>(), Int<4>(), Int<16>(), Int<WIDE ? 1 : 2>());
     }
-    // Thread blocks an SM: as many as the registers of a tile let in without spilling it. Eight quads of doubles do not fit at all: two thread blocks that
-    // read 33 to 64 channels again from L2 take 50 to 80 us for (16, 64, 112, 112) where one of 16 warps that keeps them takes 62 to 91.
-    if (WIDE || a.channels <= 32) return launch_norm<rms_norm_columns_kernel<T, VEC, 4, 8, HALF ? 3 : 2>>(a.tiles, 8, 0, stream, COLUMNS, a);
-    if constexpr (!WIDE)
-    {
-        if (a.channels <= 64) return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 8, !HALF ? 2 : VEC ? 4 : 3>>(a.tiles, 8, 0, stream, COLUMNS, a);
-        return launch_norm<rms_norm_columns_kernel<T, VEC, 8, 16, HALF ? 2 : 1>>(a.tiles, 16, 0, stream, COLUMNS, a);
-    }
+    // Few warps a thread block: four thread blocks of 4 warps that hide each other's barriers take 66 us for (64, 32, 112, 112) in float with residual where
+    // two of 8 took 80, and hold 64 channels well enough although they read half of them again from L2 (154 to 250 us for (32, 64, 224, 224) against
+    // 176 to 247); with 128 channels that is so of 8 warps (49 to 71 against 56 to 71 in 16), beyond no longer (140 against 135 for (64, 256, 56, 56)).
+    // In half precision, 4 and 8 warps for 64 channels: 111 and 114 us for (32, 64, 224, 224), 60 and 58 for rows of 75 * 101 pixels. In double,
+    // (16, 64, 112, 112): 50 to 81 us with 4 warps, 62 to 91 with 16 that hold all.
+    const auto launch = [&](auto warps, auto ctas) { return launch_norm<rms_norm_columns_kernel<T, VEC, warps, ctas>>(a.tiles, warps, 0, stream, COLUMNS, a); };
+    if constexpr (WIDE) return launch(Int<4>(), Int<3>());
+    else if constexpr (HALF) return a.channels <= (VEC ? 64 : 32) ? launch(Int<4>(), Int<6>()) : launch(Int<8>(), Int<3>());
+    else return a.channels <= 64 ? launch(Int<4>(), Int<4>()) : a.channels <= 128 ? launch(Int<8>(), Int<2>()) : launch(Int<16>(), Int<1>());
 }
 
 template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
@@ -73,7 +74,6 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
     constexpr const char* ROWS = "rms_norm_rows_backward_kernel";
     constexpr const char* COLUMNS = "rms_norm_columns_backward_kernel";
     const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
-    constexpr size_t FEW = gradient_slot_bytes<T, CODES>(4, 256);
     if (rows)
     {
         // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
@@ -91,27 +91,28 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
         if (split.warps == 8) return launch(AHEAD, Int<1>(), Int<4>(), Int<8>(), Int<2>());
         return launch(AHEAD, Int<1>(), Int<4>(), Int<16>(), Int<1>());
     }
-    constexpr size_t MORE = gradient_slot_bytes<T, CODES>(8, 256);
-    if (a.channels <= 32) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 1, 2>>(grid, 8, FEW, stream, COLUMNS, a);
-    if constexpr (sizeof(T) == 8)   // eight quads of doubles do not fit the registers
+    const auto launch = [&](auto held, auto warps, auto split, auto ctas) {
+        return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
+                                                                                                     COLUMNS, a);
+    };
+    constexpr bool WIDE = sizeof(T) == 8;
+    constexpr Int<WIDE ? 4 : 8> HELD;   // eight quads of doubles do not fit the registers
+    constexpr Int<32 / HELD> WARPS;
+    constexpr Int<gradient_blocks_per_sm(sizeof(T))> CTAS;
+    if (a.channels <= 32) return launch(HELD, WARPS, Int<1>(), CTAS);
+    if (a.channels <= 64) return launch(HELD, WARPS, Int<2>(), CTAS);
+    if (a.channels <= 128) return launch(HELD, WARPS, Int<4>(), CTAS);
+    if constexpr (!WIDE)
     {
-        if (a.channels <= 64) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 2, 2>>(grid, 8, FEW, stream, COLUMNS, a);
-        if (a.channels <= 128) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 4, 8, 4, 2>>(grid, 8, FEW, stream, COLUMNS, a);
-    }
-    else
-    {
-        if (a.channels <= 64) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 1, 2>>(grid, 8, MORE, stream, COLUMNS, a);
-        if (a.channels <= 128) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 2, 2>>(grid, 8, MORE, stream, COLUMNS, a);
-        if (a.channels <= 256) return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 8, 4, 2>>(grid, 8, MORE, stream, COLUMNS, a);
-        if (a.channels <= 512)
-            return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, 8, 16, 4, 1>>(grid, 16, gradient_slot_bytes<T, CODES>(8, 512), stream, COLUMNS, a);
+        if (a.channels <= 256) return launch(HELD, Int<8>(), Int<4>(), Int<2>());
+        if (a.channels <= 512) return launch(HELD, Int<16>(), Int<4>(), Int<1>());
     }
     return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
 }
 
 template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
-    const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T) == 8);
+    const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T));
     const int rc = backward_sums<T, VEC, CODES>(a, rows, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
     norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(

@@ -21,8 +21,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor = None, residual: torch.Tenso
         behind the norm (`checkpoint_8bit(layer, y, ..., packed=...)`).
     Returns y, the 8-bit form, or both of them; with a residual also s: (y, s), (packed, s) or (y, packed, s).
 
-    In float32 and float64 the mean and the factor are held in double and y is rounded once, so that the codes do not depend on how the sum
-    was split; in float16 and bfloat16 the sum and the factor are float32.
+    The mean and the factor are held in double and y is rounded once, so that the codes do not depend on how the sum was split.
     Differentiable once in x, residual and weight; the 8-bit form has no gradient, so 'float' or 'both' in training.
     """
     try:

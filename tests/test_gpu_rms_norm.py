@@ -131,6 +131,19 @@ def test_rows_that_share_warps_and_warps_that_share_rows(rows, channels, dtype):
         test_gradients((rows, channels), -1, dtype, keep8)
 
 
+@pytest.mark.parametrize("dtype", TYPES[:3], ids=str)
+@pytest.mark.parametrize("shape,dim", [((3, 20, 31, 33), -3), ((2, 64, 40, 40), -3), ((2, 61, 25, 41), -3), ((2, 128, 28, 28), -3), ((1, 300, 24, 24), -3), ((700, 64), -1), ((300, 250), -1),
+                                       ((64, 1024), -1), ((9, 5001), -1), ((3, 16384), -1)], ids=str)
+def test_results_are_rounded_once(shape, dim, dtype):
+    """A result is within half a step of its own binade of the value in 64 bits: what it is rounded from is off by less than 2^-40 of
+    it (46 bits of r and of the products, a sum in double), which is 2^-15 of half a step in float and less in the other types."""
+    x, r, w, s = tensors(shape, dim, dtype)
+    want = P.rms_norm(s, w, EPS, dim)
+    got = F.rms_norm(*cuda(x, w, r), eps=EPS, dim=dim)[0].cpu().double()
+    binade = torch.exp2(torch.floor(torch.log2(want.abs().clamp(min=torch.finfo(dtype).smallest_normal))))
+    assert bool(((got - want).abs() <= binade * (torch.finfo(dtype).eps / 2) * (1 + 2.0 ** -14)).all())
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
 @pytest.mark.parametrize("shape,dim", [((35, 40), -1), ((35, 128), -1), ((19, 250), -1), ((5, 700), -1), ((21, 700), -1), ((2, 9, 13, 12), -3), ((2, 70, 13, 11), -3), ((1, 600, 6, 6), -3)], ids=str)
 def test_nothing_of_a_neighbour(shape, dim, dtype):
