@@ -9,7 +9,7 @@
 // them: a forward pass with residual moves 16 bytes an element in float (13 with the result in 8 bits), a backward pass 16 (13).
 //
 // The forward pass takes the sums over the channels in double and rounds y once, from an unevaluated sum of two floats that carries
-// about 46 bits (from double in double): y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
+// about 46 bits (to float, and from there, in half precision; in double after each product): y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
 // in whatever order. A float that is one unit off moves one code in 10^5 to its neighbour; plain float arithmetic behind a result of 11 bits
 // moves one result in 2^10, and with the largest of a block its scale ((32, 64, 224, 224) in bfloat16 98 us so, 111 as it is).
 #pragma once
