@@ -4,9 +4,9 @@
 //     s = T(x + residual),  r = 1 / sqrt(mean_c s^2 + eps),  y = T(s r weight_c)
 //     gx = r (u - s r^2 mean_c(u s)) + gsum,  u = gy weight_c;   gweight_c = sum over the pixels of gy s r
 //
-// Every kernel reads its inputs once: the tile of a thread block, all channels of 128 neighbouring pixels (columns) or whole
-// rows of channels (rows), stays in registers between the sums over the channels and what is computed from them. Bytes bound
-// them: a forward pass with residual moves 16 bytes an element in float (13 with the result in 8 bits), a backward pass 16 (13).
+// Every kernel reads its inputs from memory once: the tile of a thread block, all channels of 32 to 128 neighbouring pixels (columns) or whole
+// rows of channels (rows), stays in registers, or in L2 where it has too many channels, between the sums over the channels and what is computed
+// from them. Bytes bound them: a forward pass with residual moves 16 bytes an element in float (13 with the result in 8 bits), a backward pass 16 (13).
 //
 // The forward pass takes the sums over the channels in double and rounds y once, from an unevaluated sum of two floats that carries
 // about 46 bits (to float, and from there, in half precision; in double after each product): y, and with it every code of its 8-bit form, is then what 64-bit arithmetic gives, whichever kernel computed it and
@@ -220,7 +220,7 @@ template <bool VEC, typename Args> __device__ __forceinline__ Place place_of(con
 
 /// Forward, feature maps. A block of WARPS warps takes 128 pixels of an image; warp w has the channels w, w + WARPS, ... and keeps
 /// up to eight of them. Where there are more, the second pass reads s again, from `sum` or x: the tiles that are at work then
-/// lie in L2 (128 pixels of 512 channels in float are 256 KiB, of 296 thread blocks 76 MiB).
+/// lie in L2 (128 pixels of 64 channels in float are 32 KiB, of 592 thread blocks 19 MiB; of 512 channels, of 148 thread blocks, 38 MiB).
 template <typename T, bool VEC, int WARPS, int CTAS> __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
 {
     constexpr int HELD = 8;
