@@ -144,7 +144,7 @@ template <int N, int SUMS, typename T> __device__ __forceinline__ void add_squar
 }
 
 /// Codes and scales of N blocks: block i lies `offset(i)` elements and i `block_step` blocks behind the first, whose codes and scale go to `codes`
-/// and `scales`; `count` exist.
+/// and `scales`; `count` exist from it on, of which the N here are stored: lanes beyond them have no scale, and one place is not to be written by two lanes.
 template <bool VEC, int N, typename T, typename Offset>
 __device__ __forceinline__ void put_codes(int8_t* codes, void* scales, Offset offset, int64_t block_step, const Quad<T> (&q)[N], int count, int lane, const int (&left)[N])
 {
@@ -155,7 +155,7 @@ __device__ __forceinline__ void put_codes(int8_t* codes, void* scales, Offset of
     const Wide<T> scale = encode_blocks(v, c, lane);
 #pragma unroll
     for (int i = 0; i < N; i++) store_codes<VEC>(codes + offset(i), c[i], left[i]);
-    if (lane < count) static_cast<Wide<T>*>(scales)[lane * block_step] = scale;
+    if (lane < min(count, N)) static_cast<Wide<T>*>(scales)[lane * block_step] = scale;
 }
 
 // The kernels that keep a tile in registers fetch the next one meanwhile, by asynchronous copies into slots of shared memory that only
