@@ -5,9 +5,10 @@ import ctypes
 import pytest
 import torch
 
+import _plain8 as P
 import morphocore_b200.functional as F
 from test_activation8 import Norm
-from test_gpu_rms_norm import EPS, TYPES, cuda, row_dims_of, tensors
+from test_gpu_rms_norm import EPS, TYPES, cuda, grad_bound, make, row_dims_of, tensors, weight_bound, within
 
 pytestmark = pytest.mark.gpu
 
@@ -34,3 +35,34 @@ def test_scales_of_warps_with_many_blocks(shape, dim, dtype):
         check(lib.mc_rms_norm_forward(ctypes.byref(d), ptr(x), ptr(r), ptr(w), ptr(total), None, ptr(codes[0]), ptr(scales[0]), ptr(codes[1]), ptr(scales[1]), stream()))
         for c, s, p in zip(codes, scales, wants):
             assert bool((c == p.codes).all()) and bool((s == p.scales).all())
+
+
+def check_gradients(shape, dim, dtype, keep8, residual, weight, lane_terms):
+    """Gradients against 64 bits. Beside the roundings that grad_bound and weight_bound count, `lane_terms` of each: a lane adds that many squares
+    and products one after the other in float (what comes of the lanes is added in double). Either sum is then off by at most
+    lane_terms half steps of its terms' magnitudes, r by half as much, r^2 mean(u s) by twice: with r's own 2.5 lane_terms half steps of `size`."""
+    x, r, w, s = tensors(shape, dim, dtype, residual, weight)
+    gy, gs = make(shape, dtype, 4), make(shape, dtype, 5) if residual else None
+    leaves = [None if t is None else t.requires_grad_(True) for t in cuda(x, w, r)]
+    out = F.checkpoint_8bit(F.rms_norm, *leaves, EPS, dim) if keep8 else F.rms_norm(*leaves, EPS, dim)
+    at = s
+    if keep8:
+        kept = F.encode_8bit(s.cuda(), row_dims_of(x, dim))
+        at = P.decode(kept.codes.cpu(), kept.scales.cpu(), dtype)
+    want, want_w, size, size_w = P.rms_norm_backward(at, w, gy, gs, EPS, dim)
+    got = torch.autograd.grad(out, [t for t in leaves if t is not None], [gy.cuda(), gs.cuda()] if residual else gy.cuda())
+    more = 0 if dtype == torch.float64 else 2.5 * lane_terms * 2.0 ** -24
+    within(got[0], want, grad_bound(size, want, dtype, shape[dim]) + more * size, "x")
+    if weight:
+        within(got[1], want_w, weight_bound(size_w, want_w, dtype, channels=shape[dim]) + more * size_w, "weight")
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+def test_maps_of_many_channels(dtype, keep8):
+    """Backward passes whose sums of gweight take more and more shared memory, the smallest first: no call relies on the opt-in of one
+    with more channels before it. 1792 and 3840 channels are where double leaves 48 KiB with and without what the kernel declares."""
+    for channels in (513, 1792, 1793, 2048, 3840, 3841, 8200, 16384):
+        for inner in ((2, 2), (1, 3)):
+            for residual, weight in ((True, True), (False, True), (False, False)):
+                check_gradients((2, channels, *inner), -3, dtype, keep8, residual, weight, -(-channels // 16))
