@@ -382,14 +382,17 @@ void count_launch();
 /// erosion fields, `smooth` the smooth-merge entry points. MC_OK or a negative status with the message set.
 int validate(const mc_desc* d, bool morph, bool smooth = false);
 
-/// Opt in to more than 48 KiB of dynamic shared memory for a kernel; returns false if the device refuses.
+constexpr size_t MAX_SHARED_BYTES = 227 * 1024;
+
+/// Opt in to more than 48 KiB of dynamic shared memory for a kernel that declares none itself; returns false if the device refuses. The
+/// limit is a property of the kernel that all threads of the process share, so it is always set to the same value, all that there is: a
+/// call that set what it needs itself could lower it between another thread's opt-in and its launch.
 template <typename K> inline bool allow_shared(K kernel, size_t bytes)
 {
     if (bytes <= 48 * 1024) return true;
-    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) == cudaSuccess;
+    if (bytes > MAX_SHARED_BYTES) return false;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SHARED_BYTES)) == cudaSuccess;
 }
-
-constexpr size_t MAX_SHARED_BYTES = 227 * 1024;
 
 inline int check_launch(const char* what)
 {

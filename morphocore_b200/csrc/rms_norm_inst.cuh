@@ -14,21 +14,25 @@ constexpr int LARGEST_GRID = 0x7fffffff;
 template <int N> using Int = std::integral_constant<int, N>;
 
 /// Launches KERNEL, whose shared memory needs an opt-in where it leaves the first 48 KiB together with what the kernel declares itself: up to 34 KiB, so
-/// that the dynamic part alone says nothing. The opt-in is asked for once a device (and again for more): it is 1 us of host time.
+/// that the dynamic part alone says nothing. The opt-in is to all that the kernel can have, asked for once a device (it is 1 us of host time): threads with
+/// launches of different sizes agree on it.
 template <auto KERNEL, typename Args, typename... More>
 int launch_norm(int64_t grid, int warps, size_t shared, cudaStream_t stream, const char* what, const Args& a, More... more)
 {
     if (shared > 0)
     {
         constexpr int MAX_DEVICES = 64;
-        static std::atomic<size_t> allowed[MAX_DEVICES];
+        static std::atomic<bool> allowed[MAX_DEVICES];
         int device = 0;
         cudaError_t err = cudaGetDevice(&device);
         const bool known = err == cudaSuccess && device >= 0 && device < MAX_DEVICES;
-        if (err == cudaSuccess && !(known && allowed[device].load(std::memory_order_relaxed) >= shared))
+        if (err == cudaSuccess && !(known && allowed[device].load(std::memory_order_relaxed)))
         {
-            err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(shared));
-            if (err == cudaSuccess && known) allowed[device].store(shared, std::memory_order_relaxed);
+            cudaFuncAttributes declared;
+            err = cudaFuncGetAttributes(&declared, KERNEL);
+            if (err == cudaSuccess)
+                err = cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(MAX_SHARED_BYTES - declared.sharedSizeBytes));
+            if (err == cudaSuccess && known) allowed[device].store(true, std::memory_order_relaxed);
         }
         if (err != cudaSuccess)
         {

@@ -66,3 +66,56 @@ def test_maps_of_many_channels(dtype, keep8):
         for inner in ((2, 2), (1, 3)):
             for residual, weight in ((True, True), (False, True), (False, False)):
                 check_gradients((2, channels, *inner), -3, dtype, keep8, residual, weight, -(-channels // 16))
+
+
+def in_threads(*calls, times):
+    """Each call in a thread of its own, `times` times over; ctypes gives up the interpreter's lock meanwhile."""
+    import threading
+    failed, start = [], threading.Barrier(len(calls))
+
+    def work(call):
+        start.wait()
+        for _ in range(times):
+            rc = call()
+            if rc != 0:
+                failed.append(rc)
+
+    threads = [threading.Thread(target=work, args=(call,)) for call in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    return failed
+
+
+def test_threads_whose_launches_need_different_amounts_of_shared_memory():
+    """Two threads launch the same kernel with different amounts of shared memory, each above what needs no opt-in: none is refused, and
+    the results are those of calls one after the other."""
+    from _cabi import check, lib, make_desc, ptr, stream
+    at = stream()
+    calls, results, wants = [], [], []
+    for width in (4096, 2800):   # 72 and 52 KiB of the per-channel forward pass with codes, 5 x 5
+        x, w = torch.randn(1, 1, 8, width, device="cuda"), torch.randn(1, 1, 5, 5, device="cuda")
+        y, p = torch.empty_like(x), F.encode_8bit(x)
+        codes, scales = torch.empty_like(p.codes), torch.empty_like(p.scales)
+        d = make_desc("dilation", x, w, "identity")
+        calls.append(lambda d=d, t=(x, w, y, codes, scales): lib.mc_morpho_forward8(ctypes.byref(d), *map(ptr, t), at))
+        results.append((y, codes, scales))
+        wants.append((F.dilation(x, w, "identity"), p.codes, p.scales))
+    for channels in (16000, 2000):   # 160 and 50 KiB of the norm's backward pass
+        x, gy, w = (torch.randn(s, dtype=torch.float64, device="cuda") for s in ((1, channels, 2, 2), (1, channels, 2, 2), (channels,)))
+        leaves = [t.clone().requires_grad_(True) for t in (x, w)]
+        gx, gw = torch.empty_like(x), torch.empty_like(w)
+        d = norm_desc(x, -3)
+        need = lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(d), 1)
+        ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        calls.append(lambda d=d, t=(x, w, gy, gx, gw, ws), need=need: lib.mc_rms_norm_backward(
+            ctypes.byref(d), ptr(t[0]), None, None, ptr(t[1]), ptr(t[2]), None, ptr(t[3]), ptr(t[4]), ptr(t[5]), ctypes.c_size_t(need), at))
+        results.append((gx, gw))
+        wants.append(lambda leaves=leaves, gy=gy: torch.autograd.grad(F.rms_norm(*leaves), leaves, gy))
+    torch.cuda.synchronize()
+    assert in_threads(*calls, times=3000) == []
+    for got, want in zip(results, wants):
+        for a, b in zip(got, want() if callable(want) else want):
+            assert bool((a == b).all())
