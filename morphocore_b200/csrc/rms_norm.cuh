@@ -565,12 +565,35 @@ template <typename T> struct HeldSum<T, true>
     }
 };
 
-/// The two numbers that a pixel's gradients need from its sums over the channels.
+/// The two numbers that a pixel's gradients need from its sums over the channels. The square of a factor that only double holds may leave even its range.
 template <typename W> __device__ __forceinline__ void gradient_factors(double squares, double products, double per_channel, double eps, W& r, W& pull)
 {
-    const double factor = norm_factor(squares, per_channel, eps);
+    const double factor = norm_factor(squares, per_channel, eps), mean = products * per_channel;
     r = static_cast<W>(factor);
-    pull = static_cast<W>(factor * factor * (products * per_channel));
+    if (sizeof(W) == 4 || ordinary(factor)) pull = static_cast<W>(factor * factor * mean);
+    else pull = static_cast<W>(factor * (factor * mean));
+}
+
+// The kernels of the backward pass compute gradients in W from these factors. In float that needs an eps of 2^-120 or more (TINY_EPS): r is 2^60 at most
+// then, also for the pixels of zeros whose r is that of eps alone, the places of a tile that lie outside the image among them. For a smaller
+// eps in float and half precision there are variants (EXACT) that take the pixels whose factors float does not hold by way of double: an
+// infinite factor times a zero would be NaN, and one such pixel the end of all of gweight. As one kernel for every eps the rare branch cost the usual
+// ones their registers: 5 to 10 % of most shapes, (64, 256, 56, 56) from codes 113 to 146 us.
+constexpr double TINY_EPS = 0x1p-120;
+
+/// Whether a pixel's gradients may be computed from these factors in float.
+__device__ __forceinline__ bool gradients_fit(float r, float pull) { return r > 0x1p-60f && r < 0x1p60f && fabsf(pull) < 0x1p100f; }
+
+/// gx of an element and what it gives to gweight, added to `through`; the same by way of double, which holds what float does not.
+template <typename W> __device__ __forceinline__ void element_gradient(W v, W up, W g, W r, W pull, W& gx, W& through)
+{
+    gx = r * (up * g - v * pull);
+    through += up * (v * r);
+}
+template <typename W> __device__ __forceinline__ void element_gradient_in_double(W v, W up, W g, double r, double pull, W& gx, W& through)
+{
+    gx = static_cast<W>(r * (static_cast<double>(up) * static_cast<double>(g) - static_cast<double>(v) * pull));
+    through += static_cast<W>(static_cast<double>(up) * (static_cast<double>(v) * r));
 }
 
 /// gx of a lane's quad, `more` pointing to the gradient that comes past the norm.
@@ -588,9 +611,11 @@ template <bool VEC, int LANES, typename T> __device__ __forceinline__ void put_g
 
 /// The factors of a tile's pixels in the backward kernels, r and the pull of the sum, in shared memory for all threads. `add_up` adds squares and
 /// products of the warp's channels up in the type that it is given, and again in double where float's range was left: squares and products in
-/// turn then, because the room is that of both in float. Ends with a barrier.
-template <bool VEC, int LANES, typename W, int GROUPS, int PIXELS, typename AddUp>
-__device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXELS], W (&factors)[2][PIXELS], double per_channel, double eps, int lane, int group, AddUp add_up)
+/// turn then, because the room is that of both in float. EXACT: false where some factors do not fit float, and `exact` has all of them in double
+/// then. Ends with a barrier.
+template <bool VEC, int LANES, bool EXACT, typename W, int GROUPS, int PIXELS, int PLACES, typename AddUp>
+__device__ __forceinline__ bool tile_gradient_factors(W (&part)[2][GROUPS][PIXELS], W (&factors)[2][PIXELS], double (&exact)[2][PLACES], double per_channel, double eps, int lane,
+                                                      int group, AddUp add_up)
 {
     W sums[2][4] = {};
     add_up(sums);
@@ -601,10 +626,11 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
         part[1][group][quad_at<VEC, LANES>(lane, k)] = sums[1][k];
     }
     __syncthreads();
-    bool again = false;
+    bool again = false, fits = true;
+    double total[2];
     if (threadIdx.x < PIXELS)
     {
-        double total[2] = {};
+        total[0] = total[1] = 0.0;
 #pragma unroll
         for (int g = 0; g < GROUPS; g++)
         {
@@ -613,26 +639,32 @@ __device__ __forceinline__ void tile_gradient_factors(W (&part)[2][GROUPS][PIXEL
         }
         gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
         again = out_of_range(total[0], total[1], eps);
+        if constexpr (EXACT) fits = gradients_fit(factors[0][threadIdx.x], factors[1][threadIdx.x]);
     }
     if constexpr (sizeof(W) == 8) __syncthreads();
-    else if (__syncthreads_or(again))   // for the pixels that need it: no result depends on what its neighbours hold
+    else if (__syncthreads_or(again || !fits))   // for the pixels that need it: no result depends on what its neighbours hold
     {
         rarely();
-        double exact[2][4] = {}, total[2] = {};
-        add_up(exact);
+        double sums_again[2][4] = {}, total_again[2] = {};
+        add_up(sums_again);
         double(*const wide)[PIXELS] = reinterpret_cast<double(*)[PIXELS]>(&part[0][0][0]);   // [GROUPS][PIXELS]
         for (int q = 0; q < 2; q++)
         {
 #pragma unroll
-            for (int k = 0; k < 4; k++) wide[group][quad_at<VEC, LANES>(lane, k)] = q == 0 ? exact[0][k] : exact[1][k];
+            for (int k = 0; k < 4; k++) wide[group][quad_at<VEC, LANES>(lane, k)] = q == 0 ? sums_again[0][k] : sums_again[1][k];
             __syncthreads();
             if (again)
-                for (int g = 0; g < GROUPS; g++) total[q] += wide[g][threadIdx.x];
+                for (int g = 0; g < GROUPS; g++) total_again[q] += wide[g][threadIdx.x];
             __syncthreads();
         }
-        if (again) gradient_factors(total[0], total[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        if (again) gradient_factors(total_again[0], total_again[1], per_channel, eps, factors[0][threadIdx.x], factors[1][threadIdx.x]);
+        if constexpr (EXACT)
+            if (threadIdx.x < PIXELS)
+                gradient_factors(again ? total_again[0] : total[0], again ? total_again[1] : total[1], per_channel, eps, exact[0][threadIdx.x], exact[1][threadIdx.x]);
         __syncthreads();
+        return false;
     }
+    return true;
 }
 
 /// Adds squares and products of a quad to sums of type A.
@@ -646,16 +678,22 @@ template <typename A, typename W> __device__ __forceinline__ void add_products(A
     }
 }
 
-/// gx of a quad, and the sum over its elements of what they give to gweight.
-template <typename W>
-__device__ __forceinline__ W quad_gradient(const W (&v)[4], const W (&up)[4], W g, const W (&r)[4], const W (&pull)[4], W (&gx)[4])
+/// gx of a quad, and the sum over its elements of what they give to gweight; `fit` and `exact` as tile_gradient_factors left them.
+template <bool VEC, int LANES, bool EXACT, typename W, int PLACES>
+__device__ __forceinline__ W quad_gradient(const W (&v)[4], const W (&up)[4], W g, const W (&r)[4], const W (&pull)[4], bool fit, const double (&exact)[2][PLACES], int lane, W (&gx)[4])
 {
     W through = 0;
 #pragma unroll
     for (int k = 0; k < 4; k++)
     {
-        gx[k] = r[k] * (up[k] * g - v[k] * pull[k]);
-        through += up[k] * (v[k] * r[k]);
+        if constexpr (EXACT)
+            if (!fit && !gradients_fit(r[k], pull[k]))
+            {
+                const int pixel = quad_at<VEC, LANES>(lane, k);
+                element_gradient_in_double(v[k], up[k], g, exact[0][pixel], exact[1][pixel], gx[k], through);
+                continue;
+            }
+        element_gradient(v[k], up[k], g, r[k], pull[k], gx[k], through);
     }
     return through;
 }
@@ -672,7 +710,7 @@ template <typename T, bool CODES> constexpr size_t gradient_slot_bytes(int held,
 /// 118. Three thread blocks of 4 warps with tiles of 64 pixels against two of 8 with whole ones: (32, 64, 224, 224) 257 us against 268, from codes 219
 /// against 245; in half precision, four against two: (64, 32, 112, 112) 48 against 50, from codes 50 against 57. The thread blocks walk over the tiles with
 /// gweight's sums in registers; what they have at the end leaves as one row of partial sums, which norm_weight_kernel adds up in a fixed order.
-template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int SPLIT, int CTAS>
+template <typename T, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int SPLIT, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
@@ -681,6 +719,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
     static_assert(WARPS * 32 >= PIXELS && HELD <= LANES, "a thread for every pixel of the tile, a lane for every scale");
     __shared__ W part[2][STEP][PIXELS];
     __shared__ W factors[2][PIXELS];
+    __shared__ double exact[2][EXACT ? PIXELS : 1];
     extern __shared__ __align__(16) unsigned char slots[];
     Quad<T>* const gy_slot = reinterpret_cast<Quad<T>*>(slots) + threadIdx.x;   // [HELD][threads] each
     Quad<T>* const more_slot = gy_slot + HELD * COUNT;
@@ -739,7 +778,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
             fetch(p);
         }
         fetch_commit();
-        tile_gradient_factors<VEC, LANES>(part, factors, a.per_channel, a.eps, lane, group, [&](auto& sums) {
+        const bool fit = tile_gradient_factors<VEC, LANES, EXACT>(part, factors, exact, a.per_channel, a.eps, lane, group, [&](auto& sums) {
 #pragma unroll
             for (int i = 0; i < HELD; i++)
             {
@@ -766,7 +805,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
             forget_widened(gy[i]);
             s[i].values(v);
             widen_quad(gy[i], up);
-            weight_sum[i] += quad_gradient(v, up, weight_of(i), r, pull, gx);
+            weight_sum[i] += quad_gradient<VEC, LANES, EXACT>(v, up, weight_of(i), r, pull, fit, exact, lane, gx);
             put_gradient<VEC, LANES, T>(a, gx, more_slot + i * COUNT, at, i < own ? here.left : 0);
         }
         __syncwarp();
@@ -785,13 +824,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 
 /// Backward, feature maps of more channels: the tile is read twice, the second time from L2, HELD of a warp's channels at a time, and gweight's
 /// sums live in shared memory.
-template <typename T, bool VEC, bool CODES, int HELD, int WARPS, int CTAS>
+template <typename T, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
     static_assert(WARPS >= 4, "a thread for every pixel of the tile");
     __shared__ W part[2][WARPS][CODE_BLOCK];
     __shared__ W factors[2][CODE_BLOCK];
+    __shared__ double exact[2][EXACT ? CODE_BLOCK : 1];
     extern __shared__ __align__(16) unsigned char more_shared[];
     W* const weight_sums = reinterpret_cast<W*>(more_shared);   // [channels]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, C = static_cast<int>(a.channels);
@@ -814,7 +854,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
                 gy[i] = load_quad<VEC>(static_cast<const T*>(a.gy) + at, i0 + i < own ? p.left : 0);
             }
         };
-        tile_gradient_factors<VEC, 32>(part, factors, a.per_channel, a.eps, lane, warp, [&](auto& sums) {
+        const bool fit = tile_gradient_factors<VEC, 32, EXACT>(part, factors, exact, a.per_channel, a.eps, lane, warp, [&](auto& sums) {
             for (int i0 = 0; i0 < own; i0 += HELD)
             {
                 load(i0);
@@ -852,7 +892,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
                 W v[4], up[4], gx[4];
                 s[i].values(v);
                 widen_quad(gy[i], up);
-                const W through = quad_gradient(v, up, weight_of(i0 + i), r, pull, gx);
+                const W through = quad_gradient<VEC, 32, EXACT>(v, up, weight_of(i0 + i), r, pull, fit, exact, lane, gx);
                 if (a.gweight != nullptr)
                 {
                     const W total = warp_sum(through);
@@ -871,13 +911,14 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
 
 /// Backward, rows of channels; what a warp takes next is fetched while this is computed (AHEAD: where the slots fit shared memory). gweight's
 /// sums stay in the lanes that have the channels; the groups of a thread block add theirs up in shared memory, one after the other, at the end.
-template <typename T, bool VEC, bool CODES, bool AHEAD, int ROWS, int BLOCKS, int WARPS, int CTAS>
+template <typename T, bool VEC, bool CODES, bool EXACT, bool AHEAD, int ROWS, int BLOCKS, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kernel(const NormGradArgs a, int shift)
 {
     using W = Wide<T>;
     using Held = HeldSum<T, CODES>;
     constexpr int COUNT = WARPS * 32, N = ROWS * BLOCKS;
     __shared__ double part[2][WARPS][2];
+    __shared__ double exact[EXACT ? WARPS : 1][ROWS][2];   // r and the pull of a warp's rows, where float does not hold them
     extern __shared__ __align__(16) unsigned char slots[];
     Quad<T>* const gy_slot = reinterpret_cast<Quad<T>*>(slots) + threadIdx.x;   // [N][threads] each
     Quad<T>* const more_slot = gy_slot + N * COUNT;
@@ -971,20 +1012,33 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
         };
         double total[2];
         add_up(W(0), total);
+        W r, pull;
+        bool fit = true;
         const bool again = sizeof(W) == 4 && out_of_range(total[0], total[1], a.eps);   // the warps that share a row agree
+        if constexpr (EXACT)
+        {
+            gradient_factors(total[0], total[1], a.per_channel, a.eps, r, pull);
+            fit = __all_sync(0xffffffffu, gradients_fit(r, pull));
+        }
         if (__any_sync(0xffffffffu, again))
         {
             rarely();
-            double exact[2];
-            add_up(0.0, exact);
+            double sums_again[2];
+            add_up(0.0, sums_again);
             if (again)
             {
-                total[0] = exact[0];
-                total[1] = exact[1];
+                total[0] = sums_again[0];
+                total[1] = sums_again[1];
             }
         }
-        W r, pull;
         gradient_factors(total[0], total[1], a.per_channel, a.eps, r, pull);
+        if constexpr (EXACT)
+            if (!fit)
+            {
+                __syncwarp();   // the previous rows' have been read
+                if (lane < ROWS) gradient_factors(total[0], total[1], a.per_channel, a.eps, exact[warp][lane][0], exact[warp][lane][1]);
+                __syncwarp();
+            }
         if (AHEAD) fetch_wait<1>();   // gsum is here, the next rows may travel
         W g[4];
 #pragma unroll
@@ -1003,8 +1057,13 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
 #pragma unroll
             for (int k = 0; k < 4; k++)
             {
-                gx[k] = r_row * (up[k] * g[k] - v[k] * pull_row);
-                weight_sum[q % BLOCKS][k] += up[k] * (v[k] * r_row);
+                if constexpr (EXACT)
+                    if (!fit && !gradients_fit(r_row, pull_row))
+                    {
+                        element_gradient_in_double(v[k], up[k], g[k], exact[warp][q / BLOCKS][0], exact[warp][q / BLOCKS][1], gx[k], weight_sum[q % BLOCKS][k]);
+                        continue;
+                    }
+                element_gradient(v[k], up[k], g[k], r_row, pull_row, gx[k], weight_sum[q % BLOCKS][k]);
             }
             put_gradient<VEC, 32, T>(a, gx, &more, first + t.offset(q), t.left(q, rows));
         }

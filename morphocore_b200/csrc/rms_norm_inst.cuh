@@ -73,7 +73,7 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
     else return a.channels <= 64 ? launch(Int<4>(), Int<4>()) : a.channels <= 128 ? launch(Int<8>(), Int<2>()) : launch(Int<16>(), Int<1>());
 }
 
-template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
+template <typename T, bool VEC, bool CODES, bool EXACT> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
 {
     constexpr const char* ROWS = "rms_norm_rows_backward_kernel";
     constexpr const char* COLUMNS = "rms_norm_columns_backward_kernel";
@@ -85,7 +85,7 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
         const RowSplit split = split_rows(a.tiles_per_row);
         const auto launch = [&](auto ahead, auto rows, auto blocks, auto warps, auto ctas) {
             const size_t slots = ahead ? gradient_slot_bytes<T, CODES>(rows * blocks, warps * 32) : 0;
-            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
+            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, EXACT, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
                                                                                                               split.shift);
         };
         constexpr std::true_type AHEAD;
@@ -96,7 +96,7 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
         return launch(AHEAD, Int<1>(), Int<4>(), Int<16>(), Int<1>());
     }
     const auto launch = [&](auto held, auto warps, auto split, auto ctas) {
-        return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
+        return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, EXACT, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
                                                                                                      COLUMNS, a);
     };
     constexpr bool WIDE = sizeof(T) == 8;
@@ -111,13 +111,13 @@ template <typename T, bool VEC, bool CODES> int backward_sums(const NormGradArgs
         if (a.channels <= 256) return launch(HELD, Int<8>(), Int<4>(), Int<2>());
         if (a.channels <= 512) return launch(HELD, Int<16>(), Int<4>(), Int<1>());
     }
-    return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
+    return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, EXACT, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
 }
 
-template <typename T, bool VEC, bool CODES> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
+template <typename T, bool VEC, bool CODES, bool EXACT = false> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
     const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T));
-    const int rc = backward_sums<T, VEC, CODES>(a, rows, grid, stream);
+    const int rc = backward_sums<T, VEC, CODES, EXACT>(a, rows, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
     norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(
         static_cast<const Wide<T>*>(a.partial), static_cast<T*>(a.gweight), a.channels, static_cast<int>(grid));
@@ -139,6 +139,8 @@ template <> int rms_norm_backward<MC_T>(const NormGradArgs& a, cudaStream_t stre
     using T = MC_T;
     const bool rows = a.inner == 1, codes = a.sum == nullptr;
     const bool quads = quads_fit<T>(rows ? a.channels : a.inner, {a.sum, rows ? a.weight : nullptr, a.gy, a.gsum, a.gx}, {a.sum_codes});
+    if constexpr (sizeof(T) < 8)
+        if (a.eps < TINY_EPS) return codes ? backward<T, false, true, true>(a, rows, stream) : backward<T, false, false, true>(a, rows, stream);
     if (codes) return quads ? backward<T, true, true>(a, rows, stream) : backward<T, false, true>(a, rows, stream);
     return quads ? backward<T, true, false>(a, rows, stream) : backward<T, false, false>(a, rows, stream);
 }

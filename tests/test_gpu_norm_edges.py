@@ -119,3 +119,52 @@ def test_threads_whose_launches_need_different_amounts_of_shared_memory():
     for got, want in zip(results, wants):
         for a, b in zip(got, want() if callable(want) else want):
             assert bool((a == b).all())
+
+
+EVERY_BACKWARD_KERNEL = [((2, 20, 9, 15), -3), ((3, 20, 4, 8), -3), ((2, 50, 9, 15), -3), ((2, 100, 11, 12), -3), ((1, 200, 9, 15), -3), ((1, 500, 5, 8), -3), ((1, 600, 5, 9), -3),
+                         ((35, 40), -1), ((33, 127), -1), ((19, 250), -1), ((21, 700), -1), ((3, 5000), -1), ((2, 9000), -1)]
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+@pytest.mark.parametrize("eps", [1e-60, 1e-90, 1e-200])
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("shape,dim", EVERY_BACKWARD_KERNEL, ids=str)
+def test_an_eps_that_leaves_pixels_of_zeros_a_factor_beyond_float(shape, dim, dtype, eps, keep8):
+    """A pixel of zeros, masked or padded, has r = eps^-1/2: it gives nothing to gweight, its own gradient is r u, zero where u is, infinite
+    where the type does not hold it. Tiles that hang over the image, and rows that do not fill a warp, have such places as well."""
+    _, _, w, s = tensors(shape, dim, dtype, False)
+    gy = make(shape, dtype, 4)
+    pixels, upstream = (t.transpose(dim, -1).reshape(-1, shape[dim]).clone() for t in (s, gy))
+    pixels[::3] = 0
+    upstream[::6] = 0
+    pixels[1::5] *= 2.0 ** -12 if dtype == torch.float16 else 2.0 ** -70
+    wide = list(shape)
+    wide[dim], wide[-1] = wide[-1], wide[dim]
+    s, gy = (t.reshape(wide).transpose(dim, -1).contiguous() for t in (pixels, upstream))
+    leaves = [t.requires_grad_(True) for t in cuda(s, w)]
+    y = F.checkpoint_8bit(F.rms_norm, *leaves, None, eps, dim) if keep8 else F.rms_norm(*leaves, None, eps, dim)
+    got = torch.autograd.grad(y, leaves, gy.cuda())
+    at = s
+    if keep8:
+        kept = F.encode_8bit(s.cuda(), row_dims_of(s, dim))
+        at = P.decode(kept.codes.cpu(), kept.scales.cpu(), dtype)
+    want, want_w, size, size_w = P.rms_norm_backward(at, w, gy, None, eps, dim)
+    assert bool(want_w.isfinite().all())
+    more = 0 if dtype == torch.float64 else 2.5 * -(-shape[dim] // 16) * 2.0 ** -24   # as in check_gradients
+    bound = grad_bound(size, want, dtype, shape[dim]) + more * size
+    beyond = want.abs() > torch.finfo(dtype).max   # rounds to the largest value or to infinity
+    gx = got[0].cpu().double()
+    assert not bool(gx.isnan().any())
+    assert bool(((gx - want).abs() <= bound)[~beyond].all()) and bool((gx[beyond].abs() >= torch.finfo(dtype).max).all())
+    assert bool((gx[beyond].sign() == want[beyond].sign()).all())
+    within(got[1], want_w, weight_bound(size_w, want_w, dtype, channels=shape[dim]) + more * size_w, "weight")
+
+
+def test_the_smallest_eps_in_double():
+    """r^2 leaves double's range for an eps below 2^-1024; the gradient r u of a pixel of zeros does not."""
+    for shape, dim in (((2, 5, 3, 7), -3), ((7, 40), -1), ((1, 200, 3, 3), -3)):
+        x = torch.zeros(shape, dtype=torch.float64, device="cuda", requires_grad=True)
+        w, g = torch.ones(shape[dim], dtype=torch.float64, device="cuda", requires_grad=True), make(shape, torch.float64, 4).cuda()
+        gx, gw = torch.autograd.grad(F.rms_norm(x, w, eps=1e-312, dim=dim), (x, w), g)
+        want = g.cpu() / 1e-312 ** 0.5
+        assert bool((gw == 0).all()) and bool(((gx.cpu() - want).abs() <= 8 * 2.0 ** -53 * want.abs()).all())
