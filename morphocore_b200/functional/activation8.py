@@ -50,7 +50,9 @@ def decode_8bit(packed: Activation8) -> torch.Tensor:
 class _Mode(threading.local):
     """What `checkpoint_8bit` asks of the layers that are called under it, in the calling thread."""
     active = False
-    packed = None
+    packed = None     # the 8-bit form that the caller has of `packed_of`, at that tensor's `version`
+    packed_of = None
+    version = None
 
 
 _mode = _Mode()
@@ -61,9 +63,17 @@ def keeping_8bit() -> bool:
     return _mode.active
 
 
-def kept_codes() -> tuple:
-    """Codes and scales that the caller has for the input of the layer called now, or (None, None)."""
-    return (None, None) if _mode.packed is None else (_mode.packed.codes, _mode.packed.scales)
+def _version(x):
+    """A tensor's count of changes in place, None for what has none."""
+    return x._version if isinstance(x, torch.Tensor) and not x.is_inference() else None
+
+
+def kept_codes(x: torch.Tensor = None) -> tuple:
+    """Codes and scales that the caller has for `x`, the input of the layer called now, or (None, None): they are those of one tensor, and
+    a layer that is called on another one, or on what has become of it, encodes its own. Without `x`, those of whatever tensor."""
+    if _mode.packed is None or (x is not None and (x is not _mode.packed_of or _version(x) != _mode.version)):
+        return None, None
+    return _mode.packed.codes, _mode.packed.scales
 
 
 def checkpoint_8bit(function, *args, packed: Activation8 = None, **kwargs):
@@ -77,15 +87,17 @@ def checkpoint_8bit(function, *args, packed: Activation8 = None, **kwargs):
         instead. Under torch.no_grad() nothing is kept, and nothing encoded.
     packed : the 8-bit form of the layer's input, where the caller has it already (`rms_norm` with output='both' has written it), so
         that the layer need not encode it again. For a single dilation, erosion, smorph or sigma_layer, or a module of one; it must
-        be the 8-bit form of the very input.
+        be the 8-bit form of the very input. Other layers that run meanwhile, in a module derived from one of these or in a hook, encode
+        their own inputs.
 
     The input may be changed in place, or freed, before the backward pass.
     """
     if packed is not None and not getattr(function, "takes_packed", False):
         raise ValueError("packed is the input of one layer: dilation, erosion, smorph, sigma_layer or a module of one of them")
-    before = _mode.active, _mode.packed
-    _mode.active, _mode.packed = True, packed
+    x = args[0] if args else kwargs.get("x")
+    before = _mode.active, _mode.packed, _mode.packed_of, _mode.version
+    _mode.active, _mode.packed, _mode.packed_of, _mode.version = True, packed, x, _version(x)
     try:
         return function(*args, **kwargs)
     finally:
-        _mode.active, _mode.packed = before
+        _mode.active, _mode.packed, _mode.packed_of, _mode.version = before

@@ -38,7 +38,7 @@ def sigma_layer(x: torch.Tensor, w: torch.Tensor, alpha: torch.Tensor, channel_m
         # kernel covers the case, the two separate passes otherwise; same values either way).
         modes = str_to_merge(channel_merge_mode), str_to_padding(padding_mode), padding_value, save_indices
         if keeping_8bit():
-            out_dilation, out_erosion = ops.dilation_erosion_8bit(x, w, *kept_codes(), *modes)
+            out_dilation, out_erosion = ops.dilation_erosion_8bit(x, w, *kept_codes(x), *modes)
         else:
             out_dilation, out_erosion = ops.dilation_erosion(x, w, *modes)
     else:

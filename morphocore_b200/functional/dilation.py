@@ -31,7 +31,7 @@ def dilation(x: torch.Tensor, w: torch.Tensor, channel_merge_mode: str = 'sum',
     if training and weight_dropout > 0.0:
         w = drop_weights(w, weight_dropout)
     if keeping_8bit():
-        return ops.morpho_8bit(x, w, *kept_codes(), 0, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
+        return ops.morpho_8bit(x, w, *kept_codes(x), 0, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
                                padding_value, save_indices, noise_scale if training else 0.0)
     return ops.dilation(x, w, str_to_merge(channel_merge_mode), str_to_padding(padding_mode),
                         padding_value, save_indices, noise_scale if training else 0.0)

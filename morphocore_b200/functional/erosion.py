@@ -24,7 +24,7 @@ def erosion(x: torch.Tensor, w: torch.Tensor, channel_merge_mode: str = 'sum',
         w = drop_weights(w, weight_dropout)
     noisy = training and noise_scale != 0.0
     if keeping_8bit():
-        return ops.morpho_8bit(x, w.flip((-2, -1)) if noisy else w, *kept_codes(), 1, str_to_merge(channel_merge_mode),
+        return ops.morpho_8bit(x, w.flip((-2, -1)) if noisy else w, *kept_codes(x), 1, str_to_merge(channel_merge_mode),
                                str_to_padding(padding_mode), padding_value, save_indices, noise_scale if noisy else 0.0, not noisy)
     if not noisy:
         return ops.erosion_layer(x, w, str_to_merge(channel_merge_mode), str_to_padding(padding_mode), padding_value, save_indices)

@@ -31,7 +31,7 @@ def smorph(x: torch.Tensor, w: torch.Tensor, alpha: torch.Tensor, beta: torch.Te
     else:
         merge = str_to_merge(channel_merge_mode)
     if keeping_8bit():
-        return ops.smorph_8bit(x, w, alpha, beta, *kept_codes(), merge)
+        return ops.smorph_8bit(x, w, alpha, beta, *kept_codes(x), merge)
     return ops.smorph_layer(x, w, alpha, beta, merge)
 
 

@@ -148,3 +148,24 @@ def test_signatures_and_module():
     assert m.weight.shape == (5,) and m.weight.dtype == torch.float64 and bool((m.weight == 1).all()) and set(m.state_dict()) == {"weight"}
     packed = F.Activation8(torch.zeros(2, 3, dtype=torch.int8), torch.zeros(2, 1), torch.float32)
     assert packed.shape == (2, 3) and packed.nbytes == 14
+
+
+def test_packed_belongs_to_one_tensor():
+    """The codes that a caller hands over go to layers on that very tensor, in that very state."""
+    from morphocore_b200.functional.activation8 import kept_codes
+    x, other = torch.zeros(2, 3), torch.zeros(2, 3)
+    packed = F.Activation8(torch.zeros(2, 3, dtype=torch.int8), torch.zeros(2, 1), torch.float32)
+
+    def look(x):
+        seen = [kept_codes(x), kept_codes(other), kept_codes(x.view(2, 3)), F.checkpoint_8bit(lambda x: kept_codes(x), x), kept_codes(x)]
+        x.add_(1)
+        return seen + [kept_codes(x)]
+
+    look.takes_packed = True
+    codes, no = (packed.codes, packed.scales), (None, None)
+    for call in (lambda: F.checkpoint_8bit(look, x, packed=packed), lambda: F.checkpoint_8bit(look, x=x, packed=packed)):
+        for got, want in zip(call(), (codes, no, no, no, codes, no)):
+            assert got[0] is want[0] and got[1] is want[1]
+    with torch.inference_mode():
+        inside = torch.zeros(2, 3)
+        assert F.checkpoint_8bit(look, inside, packed=packed)[0][0] is packed.codes

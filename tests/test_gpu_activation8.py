@@ -535,3 +535,37 @@ def test_per_channel_layers_through_the_c_abi():
     assert _native.launch_count() == before
     assert backward(empty) == 0 and not gw.any()
     assert forward(good) == 0 and backward(good) == 0 and _native.launch_count() == before + 3
+
+
+def test_packed_is_not_the_form_of_a_later_layer_s_input():
+    """A module derived from a layer that runs two of them, and a hook that runs one: every layer but the one on the caller's tensor encodes
+    its own input, and the gradients are those of the calls one by one."""
+    class Twice(Mnn.Dilation):
+        def forward(self, x):
+            return super().forward(super().forward(x))
+
+    layer, plain = Twice(3, 3, 3).cuda(), Mnn.Dilation(3, 3, 3).cuda()
+    torch.nn.init.normal_(layer.weight, std=0.1)
+    plain.load_state_dict(layer.state_dict())
+    x = make((2, 3, 12, 18), torch.float32, 3).cuda().requires_grad_(True)
+    packed, g = F.encode_8bit(x.detach()), make((2, 3, 12, 18), torch.float32, 4).cuda()
+
+    def one_by_one():
+        return F.checkpoint_8bit(plain, F.checkpoint_8bit(plain, x, packed=packed))
+
+    hooked = Mnn.Dilation(3, 3, 3).cuda()
+    hooked.load_state_dict(layer.state_dict())
+    hooked.register_forward_hook(lambda module, inputs, y: F.dilation(y, module.weight))
+    want = torch.autograd.grad(one_by_one(), (x, plain.weight), g)
+    for module in (layer, hooked):
+        z = F.checkpoint_8bit(module, x, packed=packed)
+        assert bool((z == one_by_one()).all())
+        for a, b in zip(torch.autograd.grad(z, (x, module.weight), g), want):
+            assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())   # atomic sums in float, as elsewhere here
+    # One 8-bit form, two layers on the same tensor.
+    w = torch.nn.Parameter(make((3, 3, 3, 3), torch.float32, 5).cuda() * 0.1)
+    alpha = torch.full((3, 3), 1.5, device="cuda")
+    both = F.checkpoint_8bit(F.erosion, x, w, packed=packed) + F.checkpoint_8bit(F.smorph, x, w, alpha, packed=packed)
+    at = F.decode_8bit(packed).requires_grad_(True)
+    for a, b in zip(torch.autograd.grad(both, (x, w), g), torch.autograd.grad(F.erosion(at, w) + F.smorph(at, w, alpha), (at, w), g)):
+        assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
