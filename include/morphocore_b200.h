@@ -218,9 +218,16 @@ typedef struct mc_norm_desc
 {
     int64_t outer, channels, inner;
     double eps;       /* > 0 */
-    int32_t dtype;    /* mc_dtype of every tensor; r and the sums are wider */
-    int32_t reserved; /* 0 */
+    int32_t dtype;    /* mc_dtype of every tensor (of the weight too, without MC_NORM_FLOAT_WEIGHT); r and the sums are wider */
+    union
+    {
+        int32_t flags;    /* mc_norm_flags, 0 for none; other bits are refused */
+        int32_t reserved; /* the field's former name */
+    };
 } mc_norm_desc;
+
+/* FLOAT_WEIGHT: weight and gweight are float beside tensors in F16 or BF16 (refused beside others). */
+enum mc_norm_flags { MC_NORM_FLOAT_WEIGHT = 1 };
 
 int mc_rms_norm_forward(const mc_norm_desc* desc, const void* x, const void* residual, const void* weight, void* sum, void* y, int8_t* y_codes,
                         void* y_scales, int8_t* sum_codes, void* sum_scales, void* stream);

@@ -29,7 +29,12 @@ int checked_norm(const mc_norm_desc* d)
         return MC_ERR_INVALID_ARGUMENT;
     }
     if (d->dtype < MC_F32 || d->dtype > MC_BF16) { set_last_error("unknown dtype %d", d->dtype); return MC_ERR_INVALID_ARGUMENT; }
-    if (d->reserved != 0) { set_last_error("reserved must be 0"); return MC_ERR_INVALID_ARGUMENT; }
+    if ((d->flags & ~MC_NORM_FLOAT_WEIGHT) != 0) { set_last_error("unknown flags 0x%x", static_cast<unsigned>(d->flags)); return MC_ERR_INVALID_ARGUMENT; }
+    if ((d->flags & MC_NORM_FLOAT_WEIGHT) != 0 && d->dtype != MC_F16 && d->dtype != MC_BF16)
+    {
+        set_last_error("MC_NORM_FLOAT_WEIGHT is for tensors in half precision, not for dtype %d", d->dtype);
+        return MC_ERR_INVALID_ARGUMENT;
+    }
     if (!(d->eps > 0.0) || d->eps > std::numeric_limits<double>::max()) { set_last_error("eps must be positive and finite, got %g", d->eps); return MC_ERR_INVALID_ARGUMENT; }
     if (d->channels > MAX_CHANNELS)
     {
@@ -56,6 +61,19 @@ int refuse(const char* why)
     return MC_ERR_INVALID_ARGUMENT;
 }
 
+/// Calls f(T{}, G{}) for the types of the tensors and of the weight.
+template <typename F> int dispatch_norm(const mc_norm_desc& d, F f)
+{
+    const bool float_weight = (d.flags & MC_NORM_FLOAT_WEIGHT) != 0;
+    return dispatch_dtype(d.dtype, [&](auto t) {
+        if constexpr (sizeof(t) == 2)
+            if (float_weight) return f(t, float{});
+        return f(t, t);
+    });
+}
+
+int weight_bytes(const mc_norm_desc& d) { return d.dtype == MC_F64 ? 8 : d.dtype == MC_F32 || (d.flags & MC_NORM_FLOAT_WEIGHT) != 0 ? 4 : 2; }
+
 int element_bytes(const mc_norm_desc& d) { return d.dtype == MC_F64 ? 8 : d.dtype == MC_F32 ? 4 : 2; }
 
 }  // namespace
@@ -81,7 +99,7 @@ int mc_rms_norm_forward(const mc_norm_desc* desc, const void* x, const void* res
     set_sizes(a, *desc);
     a.x = x; a.residual = residual; a.weight = weight; a.sum = sum; a.y = y;
     a.y_codes = y_codes; a.y_scales = y_scales; a.sum_codes = sum_codes; a.sum_scales = sum_scales;
-    return dispatch_dtype(desc->dtype, [&](auto t) { return rms_norm_forward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });
+    return dispatch_norm(*desc, [&](auto t, auto g) { return rms_norm_forward<decltype(t), decltype(g)>(a, static_cast<cudaStream_t>(stream)); });
 }
 
 size_t mc_rms_norm_backward_workspace_bytes(const mc_norm_desc* desc, int have_gweight)
@@ -99,7 +117,7 @@ int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t
     if (desc->outer * desc->inner == 0)
     {
         if (gweight == nullptr) return MC_OK;
-        const cudaError_t err = cudaMemsetAsync(gweight, 0, static_cast<size_t>(element_bytes(*desc)) * static_cast<size_t>(desc->channels), static_cast<cudaStream_t>(stream));
+        const cudaError_t err = cudaMemsetAsync(gweight, 0, static_cast<size_t>(weight_bytes(*desc)) * static_cast<size_t>(desc->channels), static_cast<cudaStream_t>(stream));
         if (err == cudaSuccess) return MC_OK;
         set_last_error("cudaMemsetAsync: %s", cudaGetErrorString(err));
         return MC_ERR_CUDA;
@@ -117,7 +135,7 @@ int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t
     set_sizes(a, *desc);
     a.sum = sum; a.sum_codes = sum_codes; a.sum_scales = sum_scales; a.weight = weight; a.gy = gy; a.gsum = gsum;
     a.gx = gx; a.gweight = gweight; a.partial = workspace;
-    return dispatch_dtype(desc->dtype, [&](auto t) { return rms_norm_backward<decltype(t)>(a, static_cast<cudaStream_t>(stream)); });
+    return dispatch_norm(*desc, [&](auto t, auto g) { return rms_norm_backward<decltype(t), decltype(g)>(a, static_cast<cudaStream_t>(stream)); });
 }
 
 }  // extern "C"

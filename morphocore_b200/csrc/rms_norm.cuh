@@ -20,6 +20,8 @@
 namespace mc
 {
 
+// T is the tensors' type throughout, G the weight's: T, or float beside half precision, as programs with float master weights have it.
+
 struct NormArgs
 {
     const void *x, *residual, *weight;
@@ -221,7 +223,7 @@ template <bool VEC, typename Args> __device__ __forceinline__ Place place_of(con
 /// Forward, feature maps. A block of WARPS warps takes 128 pixels of an image; warp w has the channels w, w + WARPS, ... and keeps
 /// up to eight of them. Where there are more, the second pass reads s again, from `sum` or x: the tiles that are at work then
 /// lie in L2 (128 pixels of 64 channels in float are 32 KiB, of 592 thread blocks 19 MiB; of 512 channels, of 148 thread blocks, 38 MiB).
-template <typename T, bool VEC, int WARPS, int CTAS> __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
+template <typename T, typename G, bool VEC, int WARPS, int CTAS> __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_kernel(const NormArgs a)
 {
     constexpr int HELD = 8;
     static_assert(WARPS >= 4 && HELD % GROUP == 0, "a thread for every pixel of the tile");
@@ -308,7 +310,7 @@ template <typename T, bool VEC, int WARPS, int CTAS> __global__ void __launch_bo
 #pragma unroll
                 for (int i = 0; i < GROUP; i++)
                 {
-                    g[i] = a.weight == nullptr || at + i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[warp + (at + i) * WARPS]);
+                    g[i] = a.weight == nullptr || at + i >= own ? W(1) : widen(static_cast<const G*>(a.weight)[warp + (at + i) * WARPS]);
                     usual = usual && ordinary_weight(g[i]);
                 }
                 Quad<T> y[GROUP];
@@ -406,7 +408,7 @@ template <bool VEC, int ROWS, int BLOCKS> struct RowTile
 /// Forward, rows of channels. Bytes bound it in float: (32768, 1024) 84 us with the residual, 97 % of the copy rate, 70 with codes. In half precision
 /// instructions do, some 20 an element: (65536, 512) in bfloat16 44 us, with residual 53 (77 %). Four thread blocks an SM: three take 48 and 58, five
 /// spill (48 and 64).
-template <typename T, bool VEC, int ROWS, int BLOCKS, int WARPS, int CTAS>
+template <typename T, typename G, bool VEC, int ROWS, int BLOCKS, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const NormArgs a, int shift)
 {
     constexpr int N = ROWS * BLOCKS;
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_kernel(const N
                 widen_quad(s[q], v);
                 if (a.weight != nullptr && (BLOCKS > 1 || q == 0))
                 {
-                    widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + q % BLOCKS * t.step, t.left_in(q % BLOCKS)), g);
+                    widen_quad(load_quad<VEC>(static_cast<const G*>(a.weight) + t.c0 + q % BLOCKS * t.step, t.left_in(q % BLOCKS)), g);
                     usual = some_ordinary && __all_sync(0xffffffffu, ordinary_weight(g[0]) && ordinary_weight(g[1]) && ordinary_weight(g[2]) && ordinary_weight(g[3]));
                 }
                 const Factor<W>& f = r[q / BLOCKS];
@@ -710,7 +712,7 @@ template <typename T, bool CODES> constexpr size_t gradient_slot_bytes(int held,
 /// 118. Three thread blocks of 4 warps with tiles of 64 pixels against two of 8 with whole ones: (32, 64, 224, 224) 257 us against 268, from codes 219
 /// against 245; in half precision, four against two: (64, 32, 112, 112) 48 against 50, from codes 50 against 57. The thread blocks walk over the tiles with
 /// gweight's sums in registers; what they have at the end leaves as one row of partial sums, which norm_weight_kernel adds up in a fixed order.
-template <typename T, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int SPLIT, int CTAS>
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int SPLIT, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
@@ -750,7 +752,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 #pragma unroll
         for (int i = 0; i < HELD; i++, at += step) fetch_quad<VEC, LANES>(more_slot + i * COUNT, static_cast<const T*>(a.gsum), at, i < own ? p.left : 0);
     };
-    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[group + i * STEP]); };
+    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const G*>(a.weight)[group + i * STEP]); };
     W weight_sum[HELD] = {};
     int64_t tile = blockIdx.x;
     Place p = place(tile);
@@ -824,7 +826,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
 
 /// Backward, feature maps of more channels: the tile is read twice, the second time from L2, HELD of a warp's channels at a time, and gweight's
 /// sums live in shared memory.
-template <typename T, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int CTAS>
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT, int HELD, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backward_kernel(const NormGradArgs a)
 {
     using W = Wide<T>;
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
     const int64_t step = WARPS * a.inner, block_step = WARPS * a.tiles_per_row;
     if (a.gweight != nullptr)
         for (int c = threadIdx.x; c < C; c += WARPS * 32) weight_sums[c] = W(0);
-    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const T*>(a.weight)[warp + i * WARPS]); };
+    const auto weight_of = [&](int i) { return a.weight == nullptr || i >= own ? W(1) : widen(static_cast<const G*>(a.weight)[warp + i * WARPS]); };
     for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x)
     {
         const Place p = place_of<VEC>(a, tile, lane, warp);
@@ -911,7 +913,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
 
 /// Backward, rows of channels; what a warp takes next is fetched while this is computed (AHEAD: where the slots fit shared memory). gweight's
 /// sums stay in the lanes that have the channels; the groups of a thread block add theirs up in shared memory, one after the other, at the end.
-template <typename T, bool VEC, bool CODES, bool EXACT, bool AHEAD, int ROWS, int BLOCKS, int WARPS, int CTAS>
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT, bool AHEAD, int ROWS, int BLOCKS, int WARPS, int CTAS>
 __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kernel(const NormGradArgs a, int shift)
 {
     using W = Wide<T>;
@@ -946,7 +948,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
         for (int q = 0; q < N; q++) fetch_quad<VEC>(more_slot + q * COUNT, static_cast<const T*>(a.gsum), row * t.C + t.c0 + t.offset(q), t.left(q, rows));
     };
     const auto weights_of = [&](int j, W (&g)[4]) {
-        if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const T*>(a.weight) + t.c0 + j * t.step, t.left_in(j)), g);
+        if (a.weight != nullptr) widen_quad(load_quad<VEC>(static_cast<const G*>(a.weight) + t.c0 + j * t.step, t.left_in(j)), g);
         else
 #pragma unroll
             for (int k = 0; k < 4; k++) g[k] = W(1);
@@ -1098,8 +1100,8 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_rows_backward_kerne
 /// gweight from the rows of partial sums, in double and in a fixed order: a thread block takes 32 channels and its 32 warps every 32nd row, many
 /// of which (592 rows at most) are in flight at once. 7.1 us with 8 warps on 444 rows of 512 channels, 4.3 us so.
 constexpr int WEIGHT_WARPS = 32;
-template <typename T>
-__global__ void __launch_bounds__(WEIGHT_WARPS * 32) norm_weight_kernel(const Wide<T>* __restrict__ partial, T* __restrict__ gweight, int64_t channels, int rows)
+template <typename G>
+__global__ void __launch_bounds__(WEIGHT_WARPS * 32) norm_weight_kernel(const Wide<G>* __restrict__ partial, G* __restrict__ gweight, int64_t channels, int rows)
 {
     __shared__ double part[WEIGHT_WARPS][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -1112,7 +1114,7 @@ __global__ void __launch_bounds__(WEIGHT_WARPS * 32) norm_weight_kernel(const Wi
     __syncthreads();
     const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + warp;   // warp w adds up channel w of the thread block
     const double total = warp_sum(part[lane][warp]);
-    if (lane == 0 && mine < channels) gweight[mine] = narrow<T>(static_cast<Wide<T>>(total));
+    if (lane == 0 && mine < channels) gweight[mine] = narrow<G>(static_cast<Wide<G>>(total));
 }
 
 }  // namespace mc

@@ -8,8 +8,9 @@ namespace mc
 struct NormArgs;
 struct NormGradArgs;
 
-template <typename T> int rms_norm_forward(const NormArgs& a, cudaStream_t stream);
-template <typename T> int rms_norm_backward(const NormGradArgs& a, cudaStream_t stream);
+/// T: the tensors' type, G: the weight's and its gradient's.
+template <typename T, typename G> int rms_norm_forward(const NormArgs& a, cudaStream_t stream);
+template <typename T, typename G> int rms_norm_backward(const NormGradArgs& a, cudaStream_t stream);
 
 /// How rows of channels are dealt out: a thread block of `warps` warps takes `rows` rows at once, 2^shift warps a row, and a warp holds `blocks` blocks
 /// of 128 channels of each of its rows. Rows of one and two blocks go four and two to a warp.

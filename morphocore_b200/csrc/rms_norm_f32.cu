@@ -1,2 +1,3 @@
 #define MC_T float
+#define MC_G float
 #include "rms_norm_inst.cuh"

@@ -1,2 +1,3 @@
 #define MC_T double
+#define MC_G double
 #include "rms_norm_inst.cuh"

@@ -1,4 +1,5 @@
-// Instantiates mc::rms_norm_forward<MC_T> and mc::rms_norm_backward<MC_T>; included by rms_norm_f32.cu, _f64, _f16 and _bf16.
+// Instantiates mc::rms_norm_forward<MC_T, MC_G> and mc::rms_norm_backward<MC_T, MC_G>; included by rms_norm_f32.cu, _f64, _f16, _bf16 and, with float
+// weights, _f16_f32 and _bf16_f32.
 #include <atomic>
 
 #include "rms_norm.cuh"
@@ -44,7 +45,7 @@ int launch_norm(int64_t grid, int warps, size_t shared, cudaStream_t stream, con
     return check_launch(what);
 }
 
-template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaStream_t stream)
+template <typename T, typename G, bool VEC> int forward(const NormArgs& a, bool rows, cudaStream_t stream)
 {
     constexpr bool WIDE = sizeof(T) == 8, HALF = sizeof(T) == 2;
     constexpr const char* ROWS = "rms_norm_rows_kernel";
@@ -53,7 +54,7 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
     {
         const RowSplit split = split_rows(a.tiles_per_row);
         const auto launch = [&](auto rows, auto blocks, auto warps, auto ctas) {
-            return launch_norm<rms_norm_rows_kernel<T, VEC, rows, blocks, warps, ctas>>((a.outer + split.rows - 1) / split.rows, warps, 0, stream, ROWS, a, split.shift);
+            return launch_norm<rms_norm_rows_kernel<T, G, VEC, rows, blocks, warps, ctas>>((a.outer + split.rows - 1) / split.rows, warps, 0, stream, ROWS, a, split.shift);
         };
         constexpr Int<WIDE ? 2 : 4> CTAS;
         if (split.blocks == 1) return launch(Int<4>(), Int<1>(), Int<8>(), CTAS);
@@ -67,13 +68,13 @@ template <typename T, bool VEC> int forward(const NormArgs& a, bool rows, cudaSt
     // 176 to 247); with 128 channels that is so of 8 warps (49 to 71 against 56 to 71 in 16), beyond no longer (140 against 135 for (64, 256, 56, 56)).
     // In half precision, 4 and 8 warps for 64 channels: 111 and 114 us for (32, 64, 224, 224), 60 and 58 for rows of 75 * 101 pixels. In double,
     // (16, 64, 112, 112): 50 to 81 us with 4 warps, 62 to 91 with 16 that hold all.
-    const auto launch = [&](auto warps, auto ctas) { return launch_norm<rms_norm_columns_kernel<T, VEC, warps, ctas>>(a.tiles, warps, 0, stream, COLUMNS, a); };
+    const auto launch = [&](auto warps, auto ctas) { return launch_norm<rms_norm_columns_kernel<T, G, VEC, warps, ctas>>(a.tiles, warps, 0, stream, COLUMNS, a); };
     if constexpr (WIDE) return launch(Int<4>(), Int<3>());
     else if constexpr (HALF) return a.channels <= (VEC ? 64 : 32) ? launch(Int<4>(), Int<6>()) : launch(Int<8>(), Int<3>());
     else return a.channels <= 64 ? launch(Int<4>(), Int<4>()) : a.channels <= 128 ? launch(Int<8>(), Int<2>()) : launch(Int<16>(), Int<1>());
 }
 
-template <typename T, bool VEC, bool CODES, bool EXACT> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
 {
     constexpr const char* ROWS = "rms_norm_rows_backward_kernel";
     constexpr const char* COLUMNS = "rms_norm_columns_backward_kernel";
@@ -85,7 +86,7 @@ template <typename T, bool VEC, bool CODES, bool EXACT> int backward_sums(const 
         const RowSplit split = split_rows(a.tiles_per_row);
         const auto launch = [&](auto ahead, auto rows, auto blocks, auto warps, auto ctas) {
             const size_t slots = ahead ? gradient_slot_bytes<T, CODES>(rows * blocks, warps * 32) : 0;
-            return launch_norm<rms_norm_rows_backward_kernel<T, VEC, CODES, EXACT, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
+            return launch_norm<rms_norm_rows_backward_kernel<T, G, VEC, CODES, EXACT, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
                                                                                                               split.shift);
         };
         constexpr std::true_type AHEAD;
@@ -96,7 +97,7 @@ template <typename T, bool VEC, bool CODES, bool EXACT> int backward_sums(const 
         return launch(AHEAD, Int<1>(), Int<4>(), Int<16>(), Int<1>());
     }
     const auto launch = [&](auto held, auto warps, auto split, auto ctas) {
-        return launch_norm<rms_norm_columns_backward_kernel<T, VEC, CODES, EXACT, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
+        return launch_norm<rms_norm_columns_backward_kernel<T, G, VEC, CODES, EXACT, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
                                                                                                      COLUMNS, a);
     };
     constexpr bool WIDE = sizeof(T) == 8;
@@ -111,38 +112,43 @@ template <typename T, bool VEC, bool CODES, bool EXACT> int backward_sums(const 
         if (a.channels <= 256) return launch(HELD, Int<8>(), Int<4>(), Int<2>());
         if (a.channels <= 512) return launch(HELD, Int<16>(), Int<4>(), Int<1>());
     }
-    return launch_norm<rms_norm_columns_twice_backward_kernel<T, VEC, CODES, EXACT, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
+    return launch_norm<rms_norm_columns_twice_backward_kernel<T, G, VEC, CODES, EXACT, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
 }
 
-template <typename T, bool VEC, bool CODES, bool EXACT = false> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT = false> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
     const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T));
-    const int rc = backward_sums<T, VEC, CODES, EXACT>(a, rows, grid, stream);
+    const int rc = backward_sums<T, G, VEC, CODES, EXACT>(a, rows, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
-    norm_weight_kernel<T><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(
-        static_cast<const Wide<T>*>(a.partial), static_cast<T*>(a.gweight), a.channels, static_cast<int>(grid));
+    norm_weight_kernel<G><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(
+        static_cast<const Wide<G>*>(a.partial), static_cast<G*>(a.gweight), a.channels, static_cast<int>(grid));
     return check_launch("norm_weight_kernel");
 }
 
+/// Whether a weight that is read as quads (rows of channels) may be.
+template <typename G> bool weight_fits(const void* weight, bool rows) { return !rows || reinterpret_cast<uintptr_t>(weight) % alignof(Quad<G>) == 0; }
+
 }  // namespace
 
-template <> int rms_norm_forward<MC_T>(const NormArgs& a, cudaStream_t stream)
+template <> int rms_norm_forward<MC_T, MC_G>(const NormArgs& a, cudaStream_t stream)
 {
     using T = MC_T;
+    using G = MC_G;
     const bool rows = a.inner == 1;
-    const bool quads = quads_fit<T>(rows ? a.channels : a.inner, {a.x, a.residual, rows ? a.weight : nullptr, a.sum, a.y}, {a.y_codes, a.sum_codes});
-    return quads ? forward<T, true>(a, rows, stream) : forward<T, false>(a, rows, stream);
+    const bool quads = quads_fit<T>(rows ? a.channels : a.inner, {a.x, a.residual, a.sum, a.y}, {a.y_codes, a.sum_codes}) && weight_fits<G>(a.weight, rows);
+    return quads ? forward<T, G, true>(a, rows, stream) : forward<T, G, false>(a, rows, stream);
 }
 
-template <> int rms_norm_backward<MC_T>(const NormGradArgs& a, cudaStream_t stream)
+template <> int rms_norm_backward<MC_T, MC_G>(const NormGradArgs& a, cudaStream_t stream)
 {
     using T = MC_T;
+    using G = MC_G;
     const bool rows = a.inner == 1, codes = a.sum == nullptr;
-    const bool quads = quads_fit<T>(rows ? a.channels : a.inner, {a.sum, rows ? a.weight : nullptr, a.gy, a.gsum, a.gx}, {a.sum_codes});
+    const bool quads = quads_fit<T>(rows ? a.channels : a.inner, {a.sum, a.gy, a.gsum, a.gx}, {a.sum_codes}) && weight_fits<G>(a.weight, rows);
     if constexpr (sizeof(T) < 8)
-        if (a.eps < TINY_EPS) return codes ? backward<T, false, true, true>(a, rows, stream) : backward<T, false, false, true>(a, rows, stream);
-    if (codes) return quads ? backward<T, true, true>(a, rows, stream) : backward<T, false, true>(a, rows, stream);
-    return quads ? backward<T, true, false>(a, rows, stream) : backward<T, false, false>(a, rows, stream);
+        if (a.eps < TINY_EPS) return codes ? backward<T, G, false, true, true>(a, rows, stream) : backward<T, G, false, false, true>(a, rows, stream);
+    if (codes) return quads ? backward<T, G, true, true>(a, rows, stream) : backward<T, G, false, true>(a, rows, stream);
+    return quads ? backward<T, G, true, false>(a, rows, stream) : backward<T, G, false, false>(a, rows, stream);
 }
 
 }  // namespace mc

@@ -1066,6 +1066,12 @@ struct NormCall
     Packed y_packed, sum_packed;
 };
 
+/// Whether a norm's weight is float32 while its tensors are in half precision: what programs with float master weights have.
+bool float_beside_half(const torch::Tensor& weight, torch::ScalarType tensors)
+{
+    return weight.defined() && weight.scalar_type() == torch::kFloat && (tensors == torch::kHalf || tensors == torch::kBFloat16);
+}
+
 NormCall run_rms_norm(const torch::Tensor& x, const torch::Tensor& residual, const torch::Tensor& weight, double eps, int64_t dim, bool want_y, bool want_codes,
                       bool keep8)
 {
@@ -1085,7 +1091,8 @@ NormCall run_rms_norm(const torch::Tensor& x, const torch::Tensor& residual, con
     {
         TORCH_CHECK(weight.dim() == 1 && weight.size(0) == x.size(dim), "weight must have shape [", x.size(dim), "], got ", weight.sizes());
         TORCH_CHECK(weight.device() == x.device(), "weight is on ", weight.device(), ", x on ", x.device());
-        TORCH_CHECK(weight.scalar_type() == x.scalar_type(), "weight must have the type of x (", x.scalar_type(), "), got ", weight.scalar_type());
+        TORCH_CHECK(weight.scalar_type() == x.scalar_type() || float_beside_half(weight, x.scalar_type()), "weight must have the type of x (", x.scalar_type(),
+                    "), or be float32 beside half precision, got ", weight.scalar_type());
     }
     const c10::cuda::CUDAGuard device_guard(x.device());
     NormCall call;
@@ -1097,6 +1104,7 @@ NormCall run_rms_norm(const torch::Tensor& x, const torch::Tensor& residual, con
     call.d.inner = product(x.sizes().slice(dim + 1));
     call.d.eps = eps;
     call.d.dtype = dtype;
+    call.d.flags = float_beside_half(weight, x.scalar_type()) ? MC_NORM_FLOAT_WEIGHT : 0;
     const auto packed_like_x = [&]() -> Packed {
         std::vector<int64_t> shape = x.sizes().slice(0, call.d.inner == 1 ? dim : dim + 1).vec();
         shape.push_back(code_blocks(call.d.inner == 1 ? call.d.channels : call.d.inner));
@@ -1172,6 +1180,7 @@ public:
                 d.inner = ctx->saved_data["inner"].toInt();
                 d.eps = ctx->saved_data["eps"].toDouble();
                 d.dtype = storage_dtype_of(gy);
+                d.flags = float_beside_half(weight, gy.scalar_type()) ? MC_NORM_FLOAT_WEIGHT : 0;
                 gx = room_like(gy);
                 const size_t ws_bytes = mc_rms_norm_backward_workspace_bytes(&d, weight.defined());
                 torch::Tensor workspace;

@@ -14,7 +14,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor = None, residual: torch.Tenso
     y = s / sqrt(mean_c s^2 + eps) * weight[c].
 
     x : float32, float64, float16 or bfloat16, CUDA; (N, C, H, W) or (C, H, W) with the default `dim`.
-    weight : (C,), optional. residual : like x, optional. All in the type of x.
+    weight : (C,), optional, in the type of x, or float32 beside an x in half precision (it then enters, and gets its gradient, unrounded).
+    residual : like x, optional, in its type.
     dim : the dimension that is normalised, at most 16384 long: -3 for the channels of feature maps, -1 for rows of channels.
     output : 'float' for y; '8bit' for its 8-bit form (an `Activation8` with a row for every plane of what follows `dim`, or for
         the channels where a single element follows), which `decode_8bit` reads; 'both' for y and that form, to be handed to the layer

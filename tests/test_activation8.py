@@ -169,3 +169,20 @@ def test_packed_belongs_to_one_tensor():
     with torch.inference_mode():
         inside = torch.zeros(2, 3)
         assert F.checkpoint_8bit(look, inside, packed=packed)[0][0] is packed.codes
+
+
+def test_norm_flags_are_refused_before_any_launch(lib):
+    """float weights go with tensors in half precision alone, and no other bit means anything."""
+    one, no = ctypes.c_void_p(16), ctypes.c_size_t(0)
+    for bad in (dict(dtype=0, reserved=1), dict(dtype=1, reserved=1), dict(dtype=2, reserved=2), dict(dtype=3, reserved=3), dict(dtype=2, reserved=-1)):
+        d = ctypes.byref(norm(**bad))
+        assert lib.mc_rms_norm_forward(d, one, None, one, None, one, None, None, None, None, None) == -1, bad
+        assert lib.mc_rms_norm_backward(d, one, None, None, one, one, None, one, one, None, no, None) == -1, bad
+        assert lib.mc_rms_norm_backward_workspace_bytes(d, 1) == 0
+    for dtype in (2, 3):
+        d = ctypes.byref(norm(dtype=dtype, reserved=1))
+        assert lib.mc_rms_norm_forward(d, None, None, one, None, one, None, None, None, None, None) == -1
+        assert lib.mc_last_error() == b"x is NULL"
+        assert lib.mc_rms_norm_backward_workspace_bytes(d, 1) == lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(norm(dtype=dtype)), 1)
+        assert lib.mc_rms_norm_backward(d, one, None, None, one, one, None, one, one, None, no, None) == -3
+    assert lib.mc_launch_count() == 0

@@ -7,8 +7,9 @@ import torch
 
 import _plain8 as P
 import morphocore_b200.functional as F
+import morphocore_b200.nn as Mnn
 from test_activation8 import Norm
-from test_gpu_rms_norm import EPS, TYPES, cuda, grad_bound, make, row_dims_of, tensors, weight_bound, within
+from test_gpu_rms_norm import EPS, TYPES, cuda, grad_bound, make, row_dims_of, tensors, value_bound, weight_bound, within
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +169,58 @@ def test_the_smallest_eps_in_double():
         gx, gw = torch.autograd.grad(F.rms_norm(x, w, eps=1e-312, dim=dim), (x, w), g)
         want = g.cpu() / 1e-312 ** 0.5
         assert bool((gw == 0).all()) and bool(((gx.cpu() - want).abs() <= 8 * 2.0 ** -53 * want.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("shape,dim", [*EVERY_BACKWARD_KERNEL, ((40, 128), -1), ((9, 256), -1), ((4, 512), -1), ((2, 4096), -1), ((2, 16384), -1), ((2, 128, 6, 6), -3)], ids=str)
+def test_float_weights_beside_half_precision(shape, dim, dtype):
+    """The weight enters unrounded, and its gradient is float32, forward and backward, from the sum and from its codes; also for a weight that
+    does not start on the boundary of a wide load."""
+    x, r, _, s = tensors(shape, dim, dtype, True, False)
+    w = make((shape[dim],), torch.float32, 3, 0.2, 1.0)
+    gy, gs = make(shape, dtype, 4), make(shape, dtype, 5)
+    more = 2.5 * -(-shape[dim] // 16) * 2.0 ** -24   # as in check_gradients
+    for offset in (0, 1):
+        for keep8 in (False, True):
+            leaves = [t.cuda().requires_grad_(True) for t in (x, torch.cat([torch.zeros(offset), w]), r)]
+            args = (leaves[0], leaves[1][offset:], leaves[2], EPS, dim)
+            with torch.no_grad():
+                coded, _ = F.rms_norm(*args, output="8bit")
+            y, total = F.checkpoint_8bit(F.rms_norm, *args) if keep8 else F.rms_norm(*args)
+            assert y.dtype == dtype and bool((total.cpu() == s).all())
+            want = P.rms_norm(s, w, EPS, dim)
+            within(y, want, value_bound(want, dtype, shape[dim]))
+            packed = F.encode_8bit(y.detach(), row_dims_of(x, dim))
+            assert bool((packed.codes == coded.codes).all()) and bool((packed.scales == coded.scales).all())
+            at = s
+            if keep8:
+                kept = F.encode_8bit(s.cuda(), row_dims_of(x, dim))
+                at = P.decode(kept.codes.cpu(), kept.scales.cpu(), dtype)
+            want, want_w, size, size_w = P.rms_norm_backward(at, w, gy, gs, EPS, dim)
+            gx, gw, _ = torch.autograd.grad((y, total), leaves, (gy.cuda(), gs.cuda()))
+            assert gx.dtype == dtype and gw.dtype == torch.float32
+            within(gx, want, grad_bound(size, want, dtype) + more * size, "x")
+            within(gw[offset:], want_w, weight_bound(size_w, want_w, torch.float32) + more * size_w, "weight")
+            # A weight that half precision holds gives what it gives in half precision.
+            short = w.to(dtype).cuda()
+            assert bool((F.rms_norm(x.cuda(), short.float(), r.cuda(), EPS, dim)[0] == F.rms_norm(x.cuda(), short, r.cuda(), EPS, dim)[0]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=str)
+def test_the_module_s_float_weight_beside_half_precision(dtype):
+    """nn.RMSNorm as it is made, with maps in half precision and a small eps, without pixels, and what is still refused."""
+    norm = Mnn.RMSNorm(6).cuda()
+    torch.nn.init.normal_(norm.weight, mean=1.0, std=0.2)
+    x, g = make((2, 6, 5, 8), dtype, 1).cuda(), make((2, 6, 5, 8), dtype, 2)
+    F.checkpoint_8bit(norm, x).backward(g.cuda())
+    assert norm.weight.grad.dtype == torch.float32 and bool(norm.weight.grad.isfinite().all())
+    empty = torch.zeros(0, 6, 5, 8, dtype=dtype, device="cuda", requires_grad=True)
+    gx, gw = torch.autograd.grad(norm(empty).sum(), (empty, norm.weight))
+    assert gx.shape == empty.shape and gw.dtype == torch.float32 and bool((gw == 0).all())
+    zeros = torch.zeros(2, 6, 5, 8, dtype=dtype, device="cuda", requires_grad=True)
+    gw, = torch.autograd.grad(F.rms_norm(zeros, norm.weight, eps=1e-90), norm.weight, g.cuda())
+    assert bool((gw == 0).all())
+    for bad, weight in ((x, norm.weight.double()), (x.float(), norm.weight.to(dtype)), (x.double(), norm.weight),
+                        (x, norm.weight.to(torch.float16 if dtype == torch.bfloat16 else torch.bfloat16))):
+        with pytest.raises(RuntimeError, match="weight must have the type of x"):
+            F.rms_norm(bad, weight)
