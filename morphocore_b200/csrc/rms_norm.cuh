@@ -719,7 +719,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
     using Held = HeldSum<T, CODES>;
     constexpr int COUNT = WARPS * 32, LANES = 32 / SPLIT, PIXELS = CODE_BLOCK / SPLIT, STEP = WARPS * SPLIT;
     static_assert(WARPS * 32 >= PIXELS && HELD <= LANES, "a thread for every pixel of the tile, a lane for every scale");
-    __shared__ W part[2][STEP][PIXELS];
+    __shared__ __align__(8) W part[2][STEP][PIXELS];   // tile_gradient_factors reads it as double as well
     __shared__ W factors[2][PIXELS];
     __shared__ double exact[2][EXACT ? PIXELS : 1];
     extern __shared__ __align__(16) unsigned char slots[];
@@ -831,7 +831,7 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_twice_backw
 {
     using W = Wide<T>;
     static_assert(WARPS >= 4, "a thread for every pixel of the tile");
-    __shared__ W part[2][WARPS][CODE_BLOCK];
+    __shared__ __align__(8) W part[2][WARPS][CODE_BLOCK];   // tile_gradient_factors reads it as double as well
     __shared__ W factors[2][CODE_BLOCK];
     __shared__ double exact[2][EXACT ? CODE_BLOCK : 1];
     extern __shared__ __align__(16) unsigned char more_shared[];
