@@ -756,9 +756,9 @@ __global__ void __launch_bounds__(WARPS * 32, CTAS) rms_norm_columns_backward_ke
     W weight_sum[HELD] = {};
     int64_t tile = blockIdx.x;
     Place p = place(tile);
-    fetch(p);
+    if (tile < tiles) fetch(p);
     fetch_commit();
-    fetch_more(p);
+    if (tile < tiles) fetch_more(p);
     fetch_commit();
     for (; tile < tiles; tile += gridDim.x)
     {

@@ -28,25 +28,43 @@ inline RowSplit split_rows(int64_t blocks)
     return {8 >> shift, 8, shift, 4};
 }
 
-/// Thread blocks an SM of the backward kernel for feature maps of up to 128 channels, whose elements have this many bytes: as many as its registers let in
-/// without spilling them.
-constexpr int gradient_blocks_per_sm(int element) { return element == 8 ? 2 : element == 4 ? 3 : 4; }
+/// Thread blocks an SM of the backward kernels for rows of channels.
+constexpr int row_gradient_blocks_per_sm(int warps) { return warps == 8 ? 2 : 1; }
+
+/// A variant of the backward kernel for feature maps that holds its tile: up to `channels` of 128 / `split` pixels, `held` by each of split * warps groups of
+/// lanes, in thread blocks of which an SM has `blocks_per_sm`. The kernel's launch and the number of its thread blocks both go by gradient_tile.
+struct GradientTile
+{
+    int channels, held, warps, split, blocks_per_sm;
+};
+/// How many variants there are for elements of so many bytes, for more and more channels; what has more channels than the last reads its tile twice. Eight quads of
+/// doubles do not fit the registers.
+constexpr int gradient_tiles(int element) { return element == 8 ? 3 : 5; }
+constexpr GradientTile gradient_tile(int element, int i)
+{
+    const int held = element == 8 ? 4 : 8, blocks_per_sm = element == 8 ? 2 : element == 4 ? 3 : 4;
+    return i < 3 ? GradientTile{32 << i, held, 32 / held, 1 << i, blocks_per_sm} : i == 3 ? GradientTile{256, held, 8, 4, 2} : GradientTile{512, held, 16, 4, 1};
+}
 
 /// Thread blocks of the backward kernels, each of which leaves one row of partial sums of gweight. They walk over the tiles (or
 /// rows): more of them than are resident would only add rows. `element`: bytes of one.
 inline int64_t norm_backward_grid(int64_t outer, int64_t channels, int64_t inner, int element)
 {
     constexpr int64_t SMS = 148;
-    if (inner != 1)
+    if (inner == 1)
     {
-        // As the launches choose: the pixels of a tile, and the thread blocks an SM.
-        const int64_t held = element == 8 ? 128 : 512;
-        const int64_t pixels = channels <= 32 ? 128 : channels <= 64 ? 64 : channels <= held ? 32 : 128;
-        const int64_t resident = channels <= 128 ? gradient_blocks_per_sm(element) : channels <= 256 && element < 8 ? 2 : 1;
-        return std::min(outer * ((inner + pixels - 1) / pixels), SMS * resident);
+        const RowSplit split = split_rows(code_blocks(channels));
+        return std::min((outer + split.rows - 1) / split.rows, SMS * row_gradient_blocks_per_sm(split.warps));
     }
-    const RowSplit split = split_rows(code_blocks(channels));
-    return std::min((outer + split.rows - 1) / split.rows, SMS * (split.warps == 8 ? 2 : 1));
+    int64_t pixels = CODE_BLOCK, resident = 1;   // of the kernel that reads its tile twice
+    for (int i = gradient_tiles(element) - 1; i >= 0; i--)
+    {
+        const GradientTile tile = gradient_tile(element, i);
+        if (channels > tile.channels) break;
+        pixels = CODE_BLOCK / tile.split;
+        resident = tile.blocks_per_sm;
+    }
+    return std::min(outer * ((inner + pixels - 1) / pixels), SMS * resident);
 }
 
 }  // namespace mc

@@ -74,51 +74,46 @@ template <typename T, typename G, bool VEC> int forward(const NormArgs& a, bool 
     else return a.channels <= 64 ? launch(Int<4>(), Int<4>()) : a.channels <= 128 ? launch(Int<8>(), Int<2>()) : launch(Int<16>(), Int<1>());
 }
 
-template <typename T, typename G, bool VEC, bool CODES, bool EXACT> int backward_sums(const NormGradArgs& a, bool rows, int64_t grid, cudaStream_t stream)
+/// Feature maps: the first variant from the Ith on that holds all channels.
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT, int I = 0> int backward_columns(const NormGradArgs& a, int64_t grid, cudaStream_t stream)
 {
-    constexpr const char* ROWS = "rms_norm_rows_backward_kernel";
-    constexpr const char* COLUMNS = "rms_norm_columns_backward_kernel";
+    if constexpr (I < gradient_tiles(sizeof(T)))
+    {
+        constexpr GradientTile TILE = gradient_tile(sizeof(T), I);
+        static_assert(TILE.held * TILE.warps * TILE.split == TILE.channels, "a place for every channel");
+        if (a.channels > TILE.channels) return backward_columns<T, G, VEC, CODES, EXACT, I + 1>(a, grid, stream);
+        return launch_norm<rms_norm_columns_backward_kernel<T, G, VEC, CODES, EXACT, TILE.held, TILE.warps, TILE.split, TILE.blocks_per_sm>>(
+            grid, TILE.warps, gradient_slot_bytes<T, CODES>(TILE.held, TILE.warps * 32), stream, "rms_norm_columns_backward_kernel", a);
+    }
+    else
+    {
+        const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
+        return launch_norm<rms_norm_columns_twice_backward_kernel<T, G, VEC, CODES, EXACT, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
+    }
+}
+
+template <typename T, typename G, bool VEC, bool CODES, bool EXACT> int backward_rows(const NormGradArgs& a, int64_t grid, cudaStream_t stream)
+{
+    // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
+    constexpr bool FITS = gradient_slot_bytes<T, CODES>(8, 512) <= 200 * 1024;
     const size_t sums = a.gweight == nullptr ? 0 : sizeof(Wide<T>) * static_cast<size_t>(a.channels);
-    if (rows)
-    {
-        // Slots, or nothing, for the rows to come; gweight's sums take their place at the end.
-        constexpr bool FITS = gradient_slot_bytes<T, CODES>(8, 512) <= 200 * 1024;
-        const RowSplit split = split_rows(a.tiles_per_row);
-        const auto launch = [&](auto ahead, auto rows, auto blocks, auto warps, auto ctas) {
-            const size_t slots = ahead ? gradient_slot_bytes<T, CODES>(rows * blocks, warps * 32) : 0;
-            return launch_norm<rms_norm_rows_backward_kernel<T, G, VEC, CODES, EXACT, ahead, rows, blocks, warps, ctas>>(grid, warps, std::max(slots, sums), stream, ROWS, a,
-                                                                                                              split.shift);
-        };
-        constexpr std::true_type AHEAD;
-        if (split.blocks == 1) return launch(AHEAD, Int<4>(), Int<1>(), Int<8>(), Int<2>());
-        if (split.blocks == 2) return launch(AHEAD, Int<2>(), Int<2>(), Int<8>(), Int<2>());
-        if (split.blocks == 8) return launch(std::bool_constant<FITS>(), Int<1>(), Int<8>(), Int<16>(), Int<1>());
-        if (split.warps == 8) return launch(AHEAD, Int<1>(), Int<4>(), Int<8>(), Int<2>());
-        return launch(AHEAD, Int<1>(), Int<4>(), Int<16>(), Int<1>());
-    }
-    const auto launch = [&](auto held, auto warps, auto split, auto ctas) {
-        return launch_norm<rms_norm_columns_backward_kernel<T, G, VEC, CODES, EXACT, held, warps, split, ctas>>(grid, warps, gradient_slot_bytes<T, CODES>(held, warps * 32), stream,
-                                                                                                     COLUMNS, a);
+    const RowSplit split = split_rows(a.tiles_per_row);
+    const auto launch = [&](auto ahead, auto rows, auto blocks, auto warps) {
+        const size_t slots = ahead ? gradient_slot_bytes<T, CODES>(rows * blocks, warps * 32) : 0;
+        return launch_norm<rms_norm_rows_backward_kernel<T, G, VEC, CODES, EXACT, ahead, rows, blocks, warps, row_gradient_blocks_per_sm(warps)>>(
+            grid, warps, std::max(slots, sums), stream, "rms_norm_rows_backward_kernel", a, split.shift);
     };
-    constexpr bool WIDE = sizeof(T) == 8;
-    constexpr Int<WIDE ? 4 : 8> HELD;   // eight quads of doubles do not fit the registers
-    constexpr Int<32 / HELD> WARPS;
-    constexpr Int<gradient_blocks_per_sm(sizeof(T))> CTAS;
-    if (a.channels <= 32) return launch(HELD, WARPS, Int<1>(), CTAS);
-    if (a.channels <= 64) return launch(HELD, WARPS, Int<2>(), CTAS);
-    if (a.channels <= 128) return launch(HELD, WARPS, Int<4>(), CTAS);
-    if constexpr (!WIDE)
-    {
-        if (a.channels <= 256) return launch(HELD, Int<8>(), Int<4>(), Int<2>());
-        if (a.channels <= 512) return launch(HELD, Int<16>(), Int<4>(), Int<1>());
-    }
-    return launch_norm<rms_norm_columns_twice_backward_kernel<T, G, VEC, CODES, EXACT, 4, 16, 1>>(grid, 16, sums, stream, "rms_norm_columns_twice_backward_kernel", a);
+    constexpr std::true_type AHEAD;
+    if (split.blocks == 1) return launch(AHEAD, Int<4>(), Int<1>(), Int<8>());
+    if (split.blocks == 2) return launch(AHEAD, Int<2>(), Int<2>(), Int<8>());
+    if (split.blocks == 8) return launch(std::bool_constant<FITS>(), Int<1>(), Int<8>(), Int<16>());
+    return split.warps == 8 ? launch(AHEAD, Int<1>(), Int<4>(), Int<8>()) : launch(AHEAD, Int<1>(), Int<4>(), Int<16>());
 }
 
 template <typename T, typename G, bool VEC, bool CODES, bool EXACT = false> int backward(const NormGradArgs& a, bool rows, cudaStream_t stream)
 {
     const int64_t grid = norm_backward_grid(a.outer, a.channels, a.inner, sizeof(T));
-    const int rc = backward_sums<T, G, VEC, CODES, EXACT>(a, rows, grid, stream);
+    const int rc = rows ? backward_rows<T, G, VEC, CODES, EXACT>(a, grid, stream) : backward_columns<T, G, VEC, CODES, EXACT>(a, grid, stream);
     if (rc != MC_OK || a.gweight == nullptr) return rc;
     norm_weight_kernel<G><<<static_cast<unsigned>((a.channels + 31) / 32), WEIGHT_WARPS * 32, 0, stream>>>(
         static_cast<const Wide<G>*>(a.partial), static_cast<G*>(a.gweight), a.channels, static_cast<int>(grid));

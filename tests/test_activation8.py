@@ -186,3 +186,17 @@ def test_norm_flags_are_refused_before_any_launch(lib):
         assert lib.mc_rms_norm_backward_workspace_bytes(d, 1) == lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(norm(dtype=dtype)), 1)
         assert lib.mc_rms_norm_backward(d, one, None, None, one, one, None, one, one, None, no, None) == -3
     assert lib.mc_launch_count() == 0
+
+
+def test_norm_gradient_thread_blocks_have_tiles(lib):
+    """A row of partial sums for every thread block of the backward pass, and a tile, or a row of channels, for each of them at least:
+    tiles are 32 to 128 pixels of an image."""
+    for dtype, size in ((0, 4), (1, 8), (2, 4), (3, 4)):
+        for channels in (1, 32, 33, 64, 65, 128, 129, 256, 257, 512, 513, 16384):
+            for outer, inner in ((1, 2), (1, 32), (3, 32), (1, 33), (2, 128), (1, 129), (100000, 3), (1, 10 ** 6)):
+                rows, rest = divmod(lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(norm(outer=outer, channels=channels, inner=inner, dtype=dtype)), 1), size * channels)
+                assert rest == 0 and outer * -(-inner // 128) >= 592 or outer * -(-inner // 128) <= rows <= outer * -(-inner // 32), (dtype, channels, outer, inner, rows)
+                assert 1 <= rows <= 592
+            for outer in (1, 5, 100000):
+                rows, rest = divmod(lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(norm(outer=outer, channels=channels, inner=1, dtype=dtype)), 1), size * channels)
+                assert rest == 0 and 1 <= rows <= min(outer, 296)
