@@ -200,3 +200,18 @@ def test_norm_gradient_thread_blocks_have_tiles(lib):
             for outer in (1, 5, 100000):
                 rows, rest = divmod(lib.mc_rms_norm_backward_workspace_bytes(ctypes.byref(norm(outer=outer, channels=channels, inner=1, dtype=dtype)), 1), size * channels)
                 assert rest == 0 and 1 <= rows <= min(outer, 296)
+
+
+def test_the_mode_is_that_of_one_thread():
+    import threading
+
+    from morphocore_b200.functional.activation8 import keeping_8bit
+    seen = []
+
+    def look():
+        other = threading.Thread(target=lambda: seen.append(keeping_8bit()))
+        other.start()
+        other.join()
+        return keeping_8bit()
+
+    assert F.checkpoint_8bit(look) and seen == [False] and not keeping_8bit()

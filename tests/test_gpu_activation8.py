@@ -569,3 +569,81 @@ def test_packed_is_not_the_form_of_a_later_layer_s_input():
     at = F.decode_8bit(packed).requires_grad_(True)
     for a, b in zip(torch.autograd.grad(both, (x, w), g), torch.autograd.grad(F.erosion(at, w) + F.smorph(at, w, alpha), (at, w), g)):
         assert bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+@pytest.mark.parametrize("k", [3, 5])
+@pytest.mark.parametrize("shape", PLANES, ids=str)
+@pytest.mark.parametrize("op", ["dilation", "erosion"])
+def test_per_channel_gradients_count_every_output_once(op, shape, k):
+    """Gradients that are whole numbers of at most 8 have sums that float holds exactly (72000 of them a channel, 2^20 at most), in any order:
+    an output that a strip or a column tile left out, or took twice, shows in either gradient as a difference."""
+    C = shape[1]
+    x, w = make(shape, torch.float32, 1), make((C, 1, k, k), torch.float32, 2) * 0.1
+    gz = torch.randint(-8, 9, shape, generator=torch.Generator().manual_seed(3)).float()
+    codes, scales, _ = P.encode(x, 2)
+    kept = P.decode(torch.from_numpy(codes), torch.from_numpy(scales), torch.float32)
+    wk = w.numpy() if op == "dilation" else np.ascontiguousarray(w.numpy()[..., ::-1, ::-1])
+    for padding in ("replicate", "geodesic", "constant"):
+        leaves = [x.cuda().requires_grad_(True), w.cuda().requires_grad_(True)]
+        z = F.checkpoint_8bit(getattr(F, op), *leaves, channel_merge_mode="identity", padding_mode=padding, padding_value=0.125)
+        got = torch.autograd.grad(z, leaves, gz.cuda())
+        gx, gw = O.morpho_backward(op, kept.numpy(), wk, gz.numpy(), "identity", padding, 0.125)
+        assert np.array_equal(got[0].cpu().numpy(), gx)
+        assert np.array_equal(got[1].cpu().numpy(), gw if op == "dilation" else gw[..., ::-1, ::-1])
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_recomputation(reentrant):
+    """Inside torch.utils.checkpoint the recomputed call keeps its input in 8 bits like the first one."""
+    from torch.utils.checkpoint import checkpoint
+    norm, layer = Mnn.RMSNorm(4).cuda(), Mnn.Dilation(4, 4, 3).cuda()
+    torch.nn.init.normal_(layer.weight, std=0.1)
+    x, g = make((2, 4, 12, 18), torch.float32, 3).cuda().requires_grad_(True), make((2, 4, 12, 18), torch.float32, 4).cuda()
+
+    def block(x):
+        return F.checkpoint_8bit(torch.nn.Sequential(norm, layer), x)
+
+    inputs = (x, norm.weight, layer.weight)
+    want = torch.autograd.grad(block(x), inputs, g)
+    y = checkpoint(block, x, use_reentrant=reentrant)
+    for t in inputs:
+        t.grad = None
+    y.backward(g)   # torch.autograd.grad does not go through the reentrant form
+    for t, b in zip(inputs, want):
+        assert bool(((t.grad - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())   # atomic sums in float, as elsewhere here
+
+
+def test_threads():
+    """Threads on streams of their own, with and without the mode, forward and backward: each gets what it gets alone."""
+    import threading
+    norm, layer = Mnn.RMSNorm(8).cuda(), Mnn.Dilation(8, 8, 3, "identity").cuda()
+    torch.nn.init.normal_(layer.weight, std=0.1)
+
+    def step(i):
+        x = make((2, 8, 20, 24 + 4 * i), torch.float32, i).cuda().requires_grad_(True)
+        y = norm(x)
+        y = F.checkpoint_8bit(layer, y) if i % 2 else layer(y)
+        packed = F.encode_8bit(y.detach())
+        return (y.detach(), packed.codes, packed.scales, *torch.autograd.grad(y, (x, norm.weight), torch.ones_like(y)))
+
+    wants, results, errors = [step(i) for i in range(4)], [None] * 4, []
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(30):
+                    results[i] = step(i)
+        except Exception as e:   # what a thread raises is lost otherwise
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for got, want in zip(results, wants):
+        for n, (a, b) in enumerate(zip(got, want)):
+            assert bool((a == b).all()) if n < 3 else bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
