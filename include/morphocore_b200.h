@@ -209,7 +209,9 @@ int mc_morpho_backward8(const mc_desc* desc, const int8_t* codes, const void* sc
  * Tensors are [outer, channels, inner], contiguous: (N, C, H * W) for feature maps, (tokens, C, 1) for rows of channels. With
  * s = x + residual rounded to the tensors' type (s = x where there is no residual),
  *     y = s * r * weight[c], r = 1 / sqrt(mean over the channels of s^2 + eps),
- * the mean and r held in double and y rounded once. y and the 8-bit forms are optional (NULL), at least one output is not. The 8-bit form is that of
+ * the mean and r held in double. In float y is rounded once, and in half precision from that float, so that y and its codes do not
+ * depend on the layout; in double the sum of the squares and each product are rounded, and y (and now and then a code) may differ in the last place
+ * between layouts. y and the 8-bit forms are optional (NULL), at least one output is not. The 8-bit form is that of
  * mc_encode8 applied to y, or to s, with rows of `inner` elements, or of `channels` where inner is 1: it is what a layer behind
  * the norm, or the norm itself, may keep for its backward pass instead of the tensor.
  * `sum` receives s; it is required with a residual and must be NULL without. Buffers that are read may not overlap those
@@ -238,7 +240,7 @@ size_t mc_rms_norm_backward_workspace_bytes(const mc_norm_desc* desc, int have_g
 /* Gradients at s, given as `sum` or (sum NULL) as its 8-bit form: with u = gy * weight[c],
  *     gx = r * (u - s r^2 mean over the channels of (u s)) + gsum, gweight[c] = sum over all but the channels of gy s r.
  * gx is the gradient of x and of the residual alike. gsum (nullable) is the gradient of the forward function's `sum`. weight
- * and gweight are NULL together or not. Results do not depend on the order in which the hardware runs the thread blocks. */
+ * and gweight are NULL together or not. A lane's share of the sums is added in float (double in double), the lanes' in double. Results do not depend on the order in which the hardware runs the thread blocks. */
 int mc_rms_norm_backward(const mc_norm_desc* desc, const void* sum, const int8_t* sum_codes, const void* sum_scales, const void* weight, const void* gy,
                          const void* gsum, void* gx, void* gweight, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -163,9 +163,9 @@ __device__ __forceinline__ void put_codes(int8_t* codes, void* scales, Offset of
 // The kernels that keep a tile in registers fetch the next one meanwhile, by asynchronous copies into slots of shared memory that only
 // the thread that issued the copy reads: no barrier and no register is spent on it, and the loads of one tile travel while the sums,
 // barriers and stores of another take their time. A slot may be fetched into again once its reader has passed a __syncwarp.
-// Backward, float, (32, 64, 224, 224): 272 us against 304 without; bfloat16 (65536, 512) rows: 75 against 103. Rows that need copies of single
-// elements lose a little ((40, 20, 75, 101): 40 against 33). The forward kernels do not
-// fetch ahead: with a residual it cost 45 us of 247, because thread blocks that stay drift apart, and neighbouring tiles, which share
+// What it gave, when thread blocks had 8 warps and whole tiles: float, (32, 64, 224, 224) 11 % of the time; bfloat16, rows of 512 channels, 27 %. Rows that need copies of single
+// elements lose a little ((40, 20, 75, 101): 40 us against 33 then, 35 now). The forward kernels do not
+// fetch ahead: with a residual it made 292 us of 247, because thread blocks that stay drift apart, and neighbouring tiles, which share
 // pages of memory, are then no longer read together.
 
 /// Bytes of `src` into shared memory, zeros where it does not exist. 4, 8 or 16 bytes.

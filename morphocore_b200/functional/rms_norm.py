@@ -22,7 +22,8 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor = None, residual: torch.Tenso
         behind the norm (`checkpoint_8bit(layer, y, ..., packed=...)`).
     Returns y, the 8-bit form, or both of them; with a residual also s: (y, s), (packed, s) or (y, packed, s).
 
-    The mean and the factor are held in double and y is rounded once, so that the codes do not depend on how the sum was split.
+    The mean and the factor are held in double. In float32 y is rounded once, in half precision from that float32, so that y and its codes
+    do not depend on strides or alignment; in float64 the last place may.
     Differentiable once in x, residual and weight; the 8-bit form has no gradient, so 'float' or 'both' in training.
     """
     try:

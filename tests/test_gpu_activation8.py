@@ -647,3 +647,16 @@ def test_threads():
     for got, want in zip(results, wants):
         for n, (a, b) in enumerate(zip(got, want)):
             assert bool((a == b).all()) if n < 3 else bool(((a - b).abs() <= 1e-4 * max(1.0, float(b.abs().max()))).all())
+
+
+def test_recomputation_outside_of_the_mode_is_refused():
+    """torch.utils.checkpoint inside the call recomputes after it, without the mode: what was kept does not match, and torch says so."""
+    from torch.utils.checkpoint import CheckpointError, checkpoint
+    x = make((2, 4, 12, 18), torch.float32, 3).cuda().requires_grad_(True)
+    alpha = torch.full((4, 4), 1.5, device="cuda", requires_grad=True)
+    w = (make((4, 4, 3, 3), torch.float32, 4) * 0.1).cuda().requires_grad_(True)
+    for call in (lambda x: F.dilation(x, w), lambda x: F.dilation(x, w, "max"), lambda x: F.erosion(x, w[:, :1], "identity"), lambda x: F.smorph(x, w, alpha),
+                 lambda x: F.sigma_layer(x, w, alpha), lambda x: F.rms_norm(x)):
+        y = F.checkpoint_8bit(lambda x: checkpoint(call, x, use_reentrant=False), x)
+        with pytest.raises(CheckpointError):
+            y.sum().backward()
