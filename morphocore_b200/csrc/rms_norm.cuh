@@ -99,7 +99,8 @@ __device__ __forceinline__ bool ordinary(double r) { return r > 0x1p-60 && r < 0
 __device__ __forceinline__ double norm_factor(double squares, double per_channel, double eps) { return rsqrt(squares * per_channel + eps); }
 
 /// Sums in float are taken once more in double where they left its range: squares near its largest value, or, for an eps that does not
-/// cover them, near its smallest; infinities and NaN.
+/// cover them, near its smallest; infinities and NaN. Products too small for float's normal numbers (upstream gradients below some 1e-33) are not: they
+/// lose digits as in any float arithmetic, and a test for them could not tell them from the zeros of a masked pixel.
 __device__ __forceinline__ bool out_of_range(double squares, double products, double eps)
 {
     return !(squares < 0x1p120) || (squares < 0x1p-60 && eps < 0x1p-60) || !(fabs(products) < 0x1p120);
